@@ -389,6 +389,67 @@ void hip_attention_decode_qk(int kv_dtype, const float* q, const float* k /*NULL
                              void* workspace /*NULL*/, size_t workspace_bytes, HipStream_t stream);
 
 /* ---------------------------------------------------------------------------------- */
+/* new, no counterpart in the reference: many sequences at once, over a paged KV cache  */
+/* or as packed prompts.                                                                */
+/* Paged cache: rows as in the contiguous caches above (row_stride elements, kv head j   */
+/* at j * head_dim), page_size of them to a page; position t of sequence s is cache row  */
+/* d_block_table[s * max_pages + t / page_size] * page_size + t % page_size.             */
+/* ---------------------------------------------------------------------------------- */
+/* The bookkeeping of a step. Sequence s (of n_seqs) has d_ctx_len[s] (NULL: 0) tokens in the
+ * cache and d_new_len[s] new ones. In the order of the sequences, the pages that their new
+ * tokens need come from d_free_pages[cursor, n_free), cursor = *d_cursor (NULL: 0), and are
+ * entered in d_block_table (other entries stay as they are). Written:
+ *   d_cu[n_seqs + 1]   tokens taken in before each sequence, and in all;
+ *   d_seq_len[n_seqs]  context and new tokens of each;
+ *   d_pos, d_slot      [n_tokens]: position and cache row of each token taken in, -1 behind
+ *                      the last (hip_qk_norm_rope_kv takes them as d_pos and d_slot, and
+ *                      skips rows of -1);
+ *   d_state[2]         the cursor behind the pages taken, and the tokens left out.
+ * Tokens are left out where room ends: the last tokens of a sequence that outgrows its table
+ * row (max_pages) or finds no free page, and those past n_tokens. Negative lengths count as 0.
+ * A table entry below 0 gives slots of -1. Outputs must not overlap inputs (d_seq_len equal to
+ * d_ctx_len or d_new_len, or d_state to d_cursor: EINVAL): a captured step takes the lengths
+ * of the step before from another buffer. max_pages * page_size <= INT32_MAX. */
+void hip_paged_plan(const int32_t* d_ctx_len /*NULL*/, const int32_t* d_new_len, int n_seqs, int page_size,
+                    int max_pages, const int32_t* d_free_pages /*NULL*/, int n_free, const int32_t* d_cursor /*NULL*/,
+                    int32_t* d_block_table, int n_tokens, int32_t* d_cu, int32_t* d_seq_len, int32_t* d_pos,
+                    int64_t* d_slot, int32_t* d_state, HipStream_t stream);
+/* Attention of the new tokens of each sequence over its pages. Tokens d_cu[s] .. d_cu[s + 1] - 1
+ * of q (d_cu NULL: token s alone, n_tokens == n_seqs) are the last of sequence s, whose
+ * d_seq_len[s] positions, those of the new tokens included, are in the cache: a token at
+ * position p attends to [max(0, p + 1 - window), p] as in hip_attention_decode. q and out
+ * [n_tokens][n_heads][head_dim] and the caches are of type dtype (F32 or BF16); sums, softmax
+ * and its state are f32; in bf16 the weights round to bf16 for their product with V in calls of
+ * many rows. Any n_heads / n_kv_heads, head_dim 64, 128, 256 or 512, any page_size.
+ * Pages outside [0, cache_pages) hold no keys; a token with no key, at a negative position or
+ * at one from min(max_len, max_pages * page_size) on gives zeros; rows of out outside
+ * [d_cu[0], d_cu[n_seqs]) stay as they are. d_cu must not fall. Keys that a token does not see
+ * do not reach it, whatever they hold. With a workspace of at least
+ * hip_attention_paged_workspace_bytes(...) bytes (16-byte aligned) long contexts are split where
+ * there are few rows; with none the call runs unsplit. The workspace holds nothing between
+ * calls; calls that overlap in time need one each. */
+size_t hip_attention_paged_workspace_bytes(int dtype, int n_seqs, int n_tokens, int max_len, int n_heads,
+                                           int n_kv_heads, int head_dim, int sliding_window);
+void hip_attention_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* out,
+                         int64_t cache_pages, int page_size, int64_t row_stride, const int32_t* d_block_table,
+                         int max_pages, const int32_t* d_cu /*NULL*/, const int32_t* d_seq_len, int n_seqs,
+                         int n_tokens, int max_len, int n_heads, int n_kv_heads, int head_dim, float attn_scale,
+                         float softcap, int sliding_window, void* workspace /*NULL*/, size_t workspace_bytes,
+                         HipStream_t stream);
+/* Attention of whole prompts, one behind the other: token i of sequence s, row d_cu[s] + i of q, k
+ * and v (d_cu NULL: one sequence of n_tokens), attends to tokens [max(0, i + 1 - window), i] of its
+ * sequence. Rows of q are q_stride elements apart, of k and v kv_stride (so they may be parts of
+ * wider rows, q_stride >= n_heads * head_dim, both multiples of 16 bytes); out is
+ * [n_tokens][n_heads][head_dim]. Types, heads, rows behind the last sequence and the workspace as in
+ * hip_attention_paged. */
+size_t hip_attention_prompt_workspace_bytes(int dtype, int n_seqs, int n_tokens, int n_heads, int n_kv_heads,
+                                            int head_dim, int sliding_window);
+void hip_attention_prompt(int dtype, const void* q, const void* k, const void* v, void* out, int64_t q_stride,
+                          int64_t kv_stride, const int32_t* d_cu /*NULL*/, int n_seqs, int n_tokens, int n_heads,
+                          int n_kv_heads, int head_dim, float attn_scale, float softcap, int sliding_window,
+                          void* workspace /*NULL*/, size_t workspace_bytes, HipStream_t stream);
+
+/* ---------------------------------------------------------------------------------- */
 /* Greedy token selection (replaces cuda_bridge.h:175) with ziglm's CPU definition      */
 /* (sampler.zig:158-170): *out_idx = first index of the greatest logit in [1, n) (index 0, */
 /* the pad token, is never chosen; NaN never compares greater; n <= 1 gives 0).          */

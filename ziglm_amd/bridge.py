@@ -130,6 +130,13 @@ SIGNATURES = {
                                             _f, _f, _i, _v]),
     "hip_attention_decode_qk": (None, [_i, _v, _v, _v, _v, _v, _i, _v, _v, _v, _i64, _i64, _v, _i64, _v, _i, _i,
                                        _i, _i, _i, _i, _i, _f, _f, _f, _i, _f, _f, _i, _v, _sz, _v]),
+    # many sequences: paged cache, packed prompts (new)
+    "hip_paged_plan": (None, [_v, _v, _i, _i, _i, _v, _i, _v, _v, _i, _v, _v, _v, _v, _v, _v]),
+    "hip_attention_paged_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "hip_attention_paged": (None, [_i, _v, _v, _v, _v, _i64, _i, _i64, _v, _i, _v, _v, _i, _i, _i, _i, _i, _i, _f, _f, _i,
+                                   _v, _sz, _v]),
+    "hip_attention_prompt_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "hip_attention_prompt": (None, [_i, _v, _v, _v, _v, _i64, _i64, _v, _i, _i, _i, _i, _i, _f, _f, _i, _v, _sz, _v]),
     "hip_geglu_ex": (None, [_i, _v, _v, _v, _i64, _v]),
     "hip_tanh_softcap_ex": (None, [_i, _v, _f, _i64, _v]),
     "hip_scale_ex": (None, [_i, _v, _f, _v, _i64, _v]),

@@ -365,6 +365,42 @@ class HipDevice:
                                        sliding_window, _ptr(d_workspace), workspace_bytes, self.stream)
         self._done("attentionDecodeQk")
 
+    # -- many sequences: paged KV cache, packed prompts (new) --------------------------------
+    def pagedPlan(self, d_ctx_len, d_new_len, n_seqs, page_size, max_pages, d_free_pages, n_free, d_cursor,
+                  d_block_table, n_tokens, d_cu, d_seq_len, d_pos, d_slot, d_state):
+        """Pages, block tables, positions and cache slots of a step's new tokens."""
+        self.b.hip_paged_plan(_ptr(d_ctx_len), _ptr(d_new_len), n_seqs, page_size, max_pages, _ptr(d_free_pages),
+                              n_free, _ptr(d_cursor), _ptr(d_block_table), n_tokens, _ptr(d_cu), _ptr(d_seq_len),
+                              _ptr(d_pos), _ptr(d_slot), _ptr(d_state), self.stream)
+        self._done("pagedPlan")
+
+    def attentionPagedWorkspaceBytes(self, dtype, n_seqs, n_tokens, max_len, n_heads, n_kv_heads, head_dim,
+                                     sliding_window=0):
+        return int(self.b.hip_attention_paged_workspace_bytes(int(dtype), n_seqs, n_tokens, max_len, n_heads,
+                                                              n_kv_heads, head_dim, sliding_window))
+
+    def attentionPaged(self, dtype, d_q, d_k_cache, d_v_cache, d_out, cache_pages, page_size, row_stride,
+                       d_block_table, max_pages, d_cu, d_seq_len, n_seqs, n_tokens, max_len, n_heads, n_kv_heads,
+                       head_dim, attn_scale, softcap, sliding_window, d_workspace=None, workspace_bytes=0):
+        """Causal attention of each sequence's new tokens over its pages; d_cu None: one token each."""
+        self.b.hip_attention_paged(int(dtype), _ptr(d_q), _ptr(d_k_cache), _ptr(d_v_cache), _ptr(d_out), cache_pages,
+                                   page_size, row_stride, _ptr(d_block_table), max_pages, _ptr(d_cu), _ptr(d_seq_len),
+                                   n_seqs, n_tokens, max_len, n_heads, n_kv_heads, head_dim, attn_scale, softcap,
+                                   sliding_window, _ptr(d_workspace), workspace_bytes, self.stream)
+        self._done("attentionPaged")
+
+    def attentionPromptWorkspaceBytes(self, dtype, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, sliding_window=0):
+        return int(self.b.hip_attention_prompt_workspace_bytes(int(dtype), n_seqs, n_tokens, n_heads, n_kv_heads,
+                                                               head_dim, sliding_window))
+
+    def attentionPrompt(self, dtype, d_q, d_k, d_v, d_out, q_stride, kv_stride, d_cu, n_seqs, n_tokens, n_heads,
+                        n_kv_heads, head_dim, attn_scale, softcap, sliding_window, d_workspace=None, workspace_bytes=0):
+        """Causal attention of packed prompts; d_cu None: one prompt."""
+        self.b.hip_attention_prompt(int(dtype), _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_out), q_stride, kv_stride,
+                                    _ptr(d_cu), n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, attn_scale, softcap,
+                                    sliding_window, _ptr(d_workspace), workspace_bytes, self.stream)
+        self._done("attentionPrompt")
+
     def gegluEx(self, dtype, d_gate, d_up, d_out, n):
         self.b.hip_geglu_ex(dtype, _ptr(d_gate), _ptr(d_up), _ptr(d_out), n, self.stream)
         self._done("gegluEx")

@@ -131,6 +131,12 @@ pub extern "c" fn hip_attention_workspace_bytes(batch: c_int, n_heads: c_int, n_
 pub extern "c" fn hip_attention_decode(kv_dtype: c_int, q: [*]const f32, k_cache: ?*const anyopaque, v_cache: ?*const anyopaque, out: [*]f32, cache_rows: i64, row_stride: i64, d_row_base: ?[*]const i64, row_base: i64, d_pos: ?[*]const i32, pos_base: c_int, max_len: c_int, batch: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, attn_scale: f32, softcap: f32, sliding_window: c_int, workspace: ?*anyopaque, workspace_bytes: usize, stream: HipStream_t) void;
 pub extern "c" fn hip_attention_decode_noalloc(kv_dtype: c_int, q: [*]const f32, k_cache: ?*const anyopaque, v_cache: ?*const anyopaque, out: [*]f32, cache_rows: i64, row_stride: i64, d_row_base: ?[*]const i64, row_base: i64, d_pos: ?[*]const i32, pos_base: c_int, max_len: c_int, batch: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, attn_scale: f32, softcap: f32, sliding_window: c_int, stream: HipStream_t) void;
 pub extern "c" fn hip_attention_decode_qk(kv_dtype: c_int, q: [*]const f32, k: ?[*]const f32, v: ?[*]const f32, q_norm_w: ?[*]const f32, k_norm_w: ?[*]const f32, v_norm: c_int, k_cache: *anyopaque, v_cache: *anyopaque, out: [*]f32, cache_rows: i64, row_stride: i64, d_row_base: ?[*]const i64, row_base: i64, d_pos: ?[*]const i32, pos_base: c_int, max_len: c_int, batch: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, rotary_dim: c_int, freq_base: f32, freq_scale: f32, eps: f32, use_unit_offset: c_int, attn_scale: f32, softcap: f32, sliding_window: c_int, workspace: ?*anyopaque, workspace_bytes: usize, stream: HipStream_t) void;
+// many sequences: paged KV cache, packed prompts (new)
+pub extern "c" fn hip_paged_plan(d_ctx_len: ?[*]const i32, d_new_len: [*]const i32, n_seqs: c_int, page_size: c_int, max_pages: c_int, d_free_pages: ?[*]const i32, n_free: c_int, d_cursor: ?[*]const i32, d_block_table: [*]i32, n_tokens: c_int, d_cu: [*]i32, d_seq_len: [*]i32, d_pos: [*]i32, d_slot: [*]i64, d_state: [*]i32, stream: HipStream_t) void;
+pub extern "c" fn hip_attention_paged_workspace_bytes(dtype: c_int, n_seqs: c_int, n_tokens: c_int, max_len: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, sliding_window: c_int) usize;
+pub extern "c" fn hip_attention_paged(dtype: c_int, q: ?*const anyopaque, k_cache: ?*const anyopaque, v_cache: ?*const anyopaque, out: ?*anyopaque, cache_pages: i64, page_size: c_int, row_stride: i64, d_block_table: [*]const i32, max_pages: c_int, d_cu: ?[*]const i32, d_seq_len: [*]const i32, n_seqs: c_int, n_tokens: c_int, max_len: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, attn_scale: f32, softcap: f32, sliding_window: c_int, workspace: ?*anyopaque, workspace_bytes: usize, stream: HipStream_t) void;
+pub extern "c" fn hip_attention_prompt_workspace_bytes(dtype: c_int, n_seqs: c_int, n_tokens: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, sliding_window: c_int) usize;
+pub extern "c" fn hip_attention_prompt(dtype: c_int, q: ?*const anyopaque, k: ?*const anyopaque, v: ?*const anyopaque, out: ?*anyopaque, q_stride: i64, kv_stride: i64, d_cu: ?[*]const i32, n_seqs: c_int, n_tokens: c_int, n_heads: c_int, n_kv_heads: c_int, head_dim: c_int, attn_scale: f32, softcap: f32, sliding_window: c_int, workspace: ?*anyopaque, workspace_bytes: usize, stream: HipStream_t) void;
 
 // greedy token selection
 pub extern "c" fn hip_argmax(logits: [*]const f32, n: c_int, out_idx: [*]c_uint, stream: HipStream_t) void;
