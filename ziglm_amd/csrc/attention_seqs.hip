@@ -9,135 +9,9 @@
 // cap > 0, softmax over t, out_h = sum_t w_t v_t; query head h reads kv head h / (n_heads / n_kv_heads).
 // Position t of a paged sequence is cache row table[s][t / page] * page + t % page; pages outside the
 // cache hold nothing and are masked. Row t of a prompt is its token cu_s + t.
-#include <math.h>
-#include <algorithm>
-
-#include "zl_common.h"
-#include "zl_host.h"
+#include "attention_seqs.h"
 
 namespace zl {
-
-typedef float acc4 __attribute__((ext_vector_type(4)));
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct SeqArgs {
-    const void* q;         // [n_tokens] rows of q_stride elements, heads of D
-    const void* kc;        // rows of kv_stride elements
-    const void* vc;
-    void* out;             // [n_tokens][nh][D]
-    float* ws;             // partials: [n_tokens][nh][nsplit][D] sums, then [..][2] (max, sum) (nsplit > 1)
-    const int32_t* cu;     // [n_seqs + 1], or null: one token a sequence (paged), one sequence (prompt)
-    const int32_t* len;    // [n_seqs] sequence lengths (paged)
-    const int32_t* table;  // [n_seqs][max_pages] (paged), or null: prompt
-    int64_t q_stride, kv_stride;
-    int64_t cache_pages;
-    int page, page_shift;  // page_shift: log2(page) or -1
-    int max_pages, max_len;
-    int n_seqs, n_tokens, nh, nkv, gq, D, window, nsplit;
-    float scale, softcap, inv_cap;
-};
-
-// The tokens of a sequence and where they stand.
-struct Seq {
-    int tok0, nq;  // first row of q, new tokens
-    int pos0;      // position of the first
-    int lim;       // positions are below this
-    int64_t row0;  // prompts: row of position 0
-    const int32_t* pages;
-};
-__device__ __forceinline__ int seq_tokens(const SeqArgs& a, int s, int& tok0) {
-    if (!a.cu) {
-        tok0 = a.table ? s : 0;
-        return a.table ? 1 : a.n_tokens;
-    }
-    tok0 = min(max(a.cu[s], 0), a.n_tokens);
-    return min(max(a.cu[s + 1], tok0), a.n_tokens) - tok0;
-}
-__device__ __forceinline__ Seq seq_of(const SeqArgs& a, int s) {
-    Seq q;
-    q.nq = seq_tokens(a, s, q.tok0);
-    if (a.table) {
-        q.pos0 = max(a.len[s], 0) - q.nq;
-        q.lim = a.max_len;
-        q.row0 = 0;
-        q.pages = a.table + (int64_t)s * a.max_pages;
-    } else {
-        q.pos0 = 0;
-        q.lim = q.nq;
-        q.row0 = q.tok0;
-        q.pages = nullptr;
-    }
-    return q;
-}
-// Cache row of position t (in range), or -1.
-__device__ __forceinline__ int row_of(const SeqArgs& a, const Seq& q, int t) {
-    if (!a.table) return (int)q.row0 + t;
-    const int e = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
-    const int id = q.pages[e];
-    return id >= 0 && id < a.cache_pages ? id * a.page + (t - e * a.page) : -1;
-}
-
-// Query rows of a kv head: row r of a sequence is token r / gq, head r % gq of the group. Tiles of R
-// consecutive rows; tile `tile` over all sequences in order -> (sequence, tile of it), or -1. Every
-// wave searches for itself, 64 sequences at a time.
-template <int R>
-__device__ __forceinline__ int find_tile(const SeqArgs& a, int tile, int& in_seq) {
-    const int lane = threadIdx.x & 63;
-    if (!a.cu) {
-        const int per = (int)(((int64_t)(a.table ? 1 : a.n_tokens) * a.gq + R - 1) / R);
-        in_seq = tile % per;
-        return tile / per < a.n_seqs ? tile / per : -1;
-    }
-    for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
-        int n = 0;
-        if (s0 + lane < a.n_seqs) {
-            int tok0;
-            n = (seq_tokens(a, s0 + lane, tok0) * a.gq + R - 1) / R;
-        }
-        int x = n;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int y = __shfl_up(x, o);
-            if (lane >= o) x += y;
-        }
-        const uint64_t past = __ballot(x > tile);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            in_seq = tile - __shfl(x - n, l);
-            return s0 + l;
-        }
-        tile -= __shfl(x, kWave - 1);
-    }
-    return -1;
-}
-
-// The keys that a tile of rows [r0, r1] sees, [ks, ke), cut into splits of whole 16-key blocks:
-// `used` splits of `chunk` keys.
-constexpr int kMinChunk = 64;
-struct Range {
-    int ks, ke, chunk, used;
-};
-__device__ __forceinline__ Range tile_range(const SeqArgs& a, const Seq& q, int r0, int r1) {
-    const int i0 = r0 / a.gq, i1 = r1 / a.gq;
-    Range g;
-    g.ke = min(q.pos0 + i1, q.lim - 1) + 1;
-    g.ks = a.window > 0 ? max(0, q.pos0 + i0 + 1 - a.window) : 0;
-    const int len = max(g.ke - g.ks, 0);
-    g.chunk = max((int)(((int64_t)len + a.nsplit - 1) / a.nsplit + 15) & ~15, kMinChunk);
-    g.used = max((int)(((int64_t)len + g.chunk - 1) / g.chunk), 1);
-    return g;
-}
-
-// 4 consecutive elements as f32
-__device__ __forceinline__ f32x4 ld4(const float* p) { return ldf4(p); }
-__device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-    return f32x4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
-}
-__device__ __forceinline__ void st4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
-__device__ __forceinline__ void st4(uint16_t* p, const f32x4& v) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-}
 
 // ---- 16 query rows on the f32 matrix cores ---------------------------------------------------
 // A workgroup takes 16 query rows of one kv head and a split of their keys, its waves the 16-key
@@ -162,12 +36,12 @@ __global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq
     id /= a.nkv;
     const int split = id % a.nsplit;
     int tile;
-    const int sq = __builtin_amdgcn_readfirstlane(find_tile<16>(a, id / a.nsplit, tile));
+    const int sq = __builtin_amdgcn_readfirstlane(find_tile<16, true>(a, id / a.nsplit, tile));
     if (sq < 0) return;
     const Seq q = seq_of(a, sq);
     const int r0 = __builtin_amdgcn_readfirstlane(tile) * 16, rows = q.nq * a.gq, r1 = min(r0 + 16, rows) - 1;
     if (r0 >= rows) return;
-    const Range rg = tile_range(a, q, r0, r1);
+    const Range rg = tile_range(a, q, r0, r1, a.nsplit);
     if (split >= rg.used) return;
     const int ks = rg.ks + split * rg.chunk, ke = min(rg.ke, ks + rg.chunk);
     const int nblk = ke > ks ? (ke - ks + 15) / 16 : 0;
@@ -377,10 +251,10 @@ __global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq
             for (int e = 0; e < 4; ++e) v[e] = L == 0.0f ? 0.0f : v[e] / L;  // (no key: zeros)
             st4((T*)a.out + (tok * a.nh + h) * D + 4 * col, v);
         } else {
-            const int64_t part = (tok * a.nh + h) * a.nsplit + split;
+            const int64_t part = (tok * a.nh + h) * a.nparts + split;
             st4(a.ws + part * D + 4 * col, v);
             if (col == 0) {
-                float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nsplit * D + 2 * part;
+                float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
                 ml[0] = M;
                 ml[1] = L;
             }
@@ -389,10 +263,10 @@ __global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq
 }
 
 // Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s, a wave
-// each. The rows' splits are those of the tile of R rows that formed them.
+// each. The row's splits are those of the tile that formed them.
 constexpr int kMaxSplits = 256;
 constexpr int kJoinWaves = 4;
-template <typename T, int D, int R>
+template <typename T, int D>
 __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     constexpr int E = D / 64;  // columns of a lane
     constexpr int PER = kMaxSplits / kWave;
@@ -415,11 +289,15 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     }
     const Seq q = seq_of(a, sq);
     if (tok < q.tok0 || tok >= q.tok0 + q.nq) return;
-    const int r = (tok - q.tok0) * a.gq + h % a.gq, r0 = r / R * R, r1 = min(r0 + R, q.nq * a.gq) - 1;
-    const Range rg = tile_range(a, q, r0, r1);
+    const int rows = q.nq * a.gq;
+    const bool few = rows <= a.few_rows;
+    const int R = few ? 16 : a.tile_rows;
+    const float unit = few ? kLog2e : a.unit;
+    const int r = (tok - q.tok0) * a.gq + h % a.gq, r0 = r / R * R, r1 = min(r0 + R, rows) - 1;
+    const Range rg = tile_range(a, q, r0, r1, few ? a.nsplit : a.tile_split);
     if (rg.used == 1) return;
-    const int64_t part = th * a.nsplit;
-    const float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nsplit * D + 2 * part;
+    const int64_t part = th * a.nparts;
+    const float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
     float mv[PER], lv[PER], M = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -433,7 +311,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     float L = 0.0f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        mv[j] = exp2f((mv[j] - (M == -INFINITY ? 0.0f : M)) * kLog2e);
+        mv[j] = exp2f((mv[j] - (M == -INFINITY ? 0.0f : M)) * unit);
         L = fmaf(lv[j], mv[j], L);
     }
     L = group_sum<kWave>(L);
@@ -459,33 +337,54 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
 
 // ---- host --------------------------------------------------------------------------------------
 
-// Tiles of R query rows over all sequences, at most: sum of ceil(new tokens * gq / R).
-static int64_t most_tiles(const SeqArgs& a, int R) {
-    return std::min<int64_t>((int64_t)a.n_tokens * a.gq / R + a.n_seqs, (int64_t)a.n_tokens * cdiv(a.gq, R));
-}
-// Splits of a tile's keys: as many as bring the launch to about 512 workgroups, none shorter than 128
-// keys of the longest possible range.
-static int choose_splits(const SeqArgs& a) {
-    const int64_t len = a.window > 0 ? std::min<int64_t>((int64_t)a.window + 15, a.max_len) : a.max_len;
-    const int64_t want = cdiv(512, std::max<int64_t>(most_tiles(a, 16) * a.nkv, 1));
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, cdiv(len, 128), (int64_t)kMaxSplits}));
-}
-static size_t split_bytes(const SeqArgs& a, int nsplit) {
-    return nsplit > 1 ? (size_t)a.n_tokens * a.nh * nsplit * (a.D + 2) * sizeof(float) : 0;
-}
-static size_t workspace_bytes_of(SeqArgs& a) {
-    if (a.n_seqs <= 0 || a.n_tokens <= 0 || a.nh <= 0 || a.nkv <= 0 || a.nh % a.nkv != 0 || a.D <= 0 || a.max_len <= 0) return 0;
+// Which kernels a call takes, and the splits of each one's ranges. k_seq_tile takes bf16 calls'
+// sequences of more than 16 query rows; a call whose sequences all have that few (a token each), or
+// surely more (a prompt, one chunk), launches one kernel only.
+// Splits: as many as bring the launch to about 512 workgroups (256 of k_seq_tile), none shorter than 128
+// (256) keys of the longest possible range.
+static void choose(SeqArgs& a, int dtype) {
     a.gq = a.nh / a.nkv;
-    return split_bytes(a, choose_splits(a));
+    a.tile_rows = tile_rows_of(a.D);
+    const bool single = a.table && !a.cu;  // a token each
+    if (dtype != HIP_BRIDGE_BF16 || (int64_t)a.n_tokens * a.gq <= 16 || (single && a.gq <= 16)) a.few_rows = INT32_MAX;
+    else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : 16;
+    auto splits = [&](int R, int wgs, int least) {
+        const int64_t len = a.window > 0 ? std::min<int64_t>((int64_t)a.window + (R - 1) / a.gq, a.max_len) : a.max_len;
+        const int64_t want = cdiv(wgs, std::max<int64_t>(most_tiles(a, R) * a.nkv, 1));
+        return (int)std::max<int64_t>(1, std::min<int64_t>({want, cdiv(len, least), (int64_t)kMaxSplits}));
+    };
+    a.nsplit = a.few_rows > 0 ? splits(16, 512, 128) : 1;
+    a.tile_split = a.few_rows < INT32_MAX ? splits(a.tile_rows, 256, 256) : 1;
+    a.nparts = std::max(a.nsplit, a.tile_split);
+}
+static size_t split_bytes(const SeqArgs& a) {
+    return a.nparts > 1 ? (size_t)a.n_tokens * a.nh * a.nparts * (a.D + 2) * sizeof(float) : 0;
+}
+static size_t workspace_bytes_of(SeqArgs& a, int dtype, bool paged) {
+    if (a.n_seqs <= 0 || a.n_tokens <= 0 || a.nh <= 0 || a.nkv <= 0 || a.nh % a.nkv != 0 || a.D <= 0 || a.max_len <= 0) return 0;
+    static const int32_t some = 0;  // (never followed)
+    a.table = paged ? &some : nullptr;
+    a.cu = &some;
+    choose(a, dtype);
+    size_t need = split_bytes(a);
+    if (paged && a.n_tokens == a.n_seqs) {  // also called without d_cu
+        a.cu = nullptr;
+        choose(a, dtype);
+        need = std::max(need, split_bytes(a));
+    }
+    return need;
 }
 
 template <typename T, int D>
 static void launch_rows(const SeqArgs& a, hipStream_t s) {
-    const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
-    k_seq_rows<T, D><<<(unsigned)grid, row_waves<D>() * kWave, 0, s>>>(a);
-    if (a.nsplit > 1) {
+    if (a.few_rows > 0) {
+        const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
+        k_seq_rows<T, D><<<(unsigned)grid, row_waves<D>() * kWave, 0, s>>>(a);
+    }
+    if (a.few_rows < INT32_MAX) launch_tiles(a, s);
+    if (a.nparts > 1) {
         const int64_t th = (int64_t)a.n_tokens * a.nh;
-        k_seq_join<T, D, 16><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
+        k_seq_join<T, D><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
     }
     check_launch();
 }
@@ -511,12 +410,13 @@ static void launch_seqs(int dtype, SeqArgs& a, void* ws, size_t ws_bytes, hipStr
         set_error(HIP_BRIDGE_EUNSUPPORTED);
         return;
     }
-    a.gq = a.nh / a.nkv;
-    a.inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
-    a.nsplit = choose_splits(a);
-    if (a.nsplit > 1 && (!ws || !aligned16(ws) || split_bytes(a, a.nsplit) > ws_bytes)) a.nsplit = 1;
+    choose(a, dtype);
+    if (a.nparts > 1 && (!ws || !aligned16(ws) || split_bytes(a) > ws_bytes)) a.nsplit = a.tile_split = a.nparts = 1;
     a.ws = (float*)ws;
-    if (most_tiles(a, 16) * a.nkv * a.nsplit > INT32_MAX) {
+    a.inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    // (never 0: a masked score of -inf times it stays -inf)
+    a.unit = std::max(a.softcap > 0.0f ? kLog2e : kLog2e * std::fabs(a.scale), 1e-30f);
+    if (most_tiles(a, 16) * a.nkv * a.nparts > INT32_MAX) {
         set_error(HIP_BRIDGE_EUNSUPPORTED);
         return;
     }
@@ -540,7 +440,7 @@ size_t hip_attention_paged_workspace_bytes(int dtype, int n_seqs, int n_tokens, 
     a.nkv = n_kv_heads;
     a.D = head_dim;
     a.window = sliding_window;
-    return workspace_bytes_of(a);
+    return workspace_bytes_of(a, dtype, true);
 }
 
 void hip_attention_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* out,
@@ -594,7 +494,7 @@ size_t hip_attention_prompt_workspace_bytes(int dtype, int n_seqs, int n_tokens,
     a.nkv = n_kv_heads;
     a.D = head_dim;
     a.window = sliding_window;
-    return workspace_bytes_of(a);
+    return workspace_bytes_of(a, dtype, false);
 }
 
 void hip_attention_prompt(int dtype, const void* q, const void* k, const void* v, void* out, int64_t q_stride,
