@@ -10,6 +10,7 @@
 namespace zl {
 
 typedef float acc4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct SeqArgs {
@@ -28,9 +29,10 @@ struct SeqArgs {
     int n_seqs, n_tokens, nh, nkv, gq, D, window;
     int few_rows;          // sequences of at most this many query rows a kv head are k_seq_rows's, the others k_seq_tile's
     int nsplit, tile_split, nparts;  // splits of k_seq_rows's and k_seq_tile's ranges, the larger of them
+    int chunk, tile_chunk;           // keys of a split
     int tile_rows;         // query rows of a workgroup of k_seq_tile
     float scale, softcap, inv_cap;
-    float unit;            // k_seq_tile: log2(e) * |scale| (soft-capped scores: log2(e))
+    float unit;            // of running maxima: log2(e); bf16: log2(e) * |scale|, or log2(e) where soft-capped
 };
 
 // The tokens of a sequence and where they stand.
@@ -108,22 +110,21 @@ __device__ __forceinline__ int find_tile(const SeqArgs& a, int tile, int& in_seq
     return -1;
 }
 
-// The keys that a tile of rows [r0, r1] sees, [ks, ke), cut into at most nsplit splits: `used` of `chunk` keys,
-// a multiple of 64.
-constexpr int kMinChunk = 64;
+// The keys that a tile of rows [r0, r1] sees, [ks, ke), in `used` splits of `chunk`.
 struct Range {
-    int ks, ke, chunk, used;
+    int ks, ke, used;
 };
-__device__ __forceinline__ Range tile_range(const SeqArgs& a, const Seq& q, int r0, int r1, int nsplit) {
+__device__ __forceinline__ Range tile_range(const SeqArgs& a, const Seq& q, int r0, int r1, int chunk) {
     const int i0 = r0 / a.gq, i1 = r1 / a.gq;
     Range g;
     g.ke = min(q.pos0 + i1, q.lim - 1) + 1;
     g.ks = a.window > 0 ? max(0, q.pos0 + i0 + 1 - a.window) : 0;
-    const int len = max(g.ke - g.ks, 0);
-    g.chunk = (int)(((int64_t)len + nsplit - 1) / nsplit + kMinChunk - 1) & ~(kMinChunk - 1);
-    g.chunk = max(g.chunk, kMinChunk);
-    g.used = max((int)(((int64_t)len + g.chunk - 1) / g.chunk), 1);
+    g.used = max((int)(((int64_t)(g.ke - g.ks) + chunk - 1) / chunk), 1);
     return g;
+}
+// The same, at most, as the host knows it: keys of a tile of R rows, and splits.
+inline int64_t most_keys(const SeqArgs& a, int R) {
+    return a.window > 0 ? std::min<int64_t>((int64_t)a.window + cdiv(R - 1, a.gq), a.max_len) : a.max_len;
 }
 
 // 4 consecutive elements as f32

@@ -13,21 +13,35 @@
 
 namespace zl {
 
-// ---- 16 query rows on the f32 matrix cores ---------------------------------------------------
-// A workgroup takes 16 query rows of one kv head and a split of their keys, its waves the 16-key
-// blocks in turn, with the f32 MFMA 16x16x4 (exact f32 products and sums; bf16 values are exact in
-// f32). Scores are formed transposed, S^T = K Q^T, so that lane (n = lane % 16, g = lane / 16) holds
-// query row n and keys 4 g + r in register r, the A operand of P V as it stands. The waves' online
-// softmax states merge through LDS.
-template <int D> constexpr int row_waves() { return D > 256 ? 4 : 8; }
+// ---- 16 query rows on the matrix cores ---------------------------------------------------------
+// Decode and short chunks: a workgroup takes 16 query rows of one kv head (or as many as there are)
+// and a split of their keys, its waves the blocks of keys in turn, K and V straight from the
+// cache into operand registers: the call is bound by reading the cache once. f32 calls take 16
+// keys to a block and the f32 MFMA 16x16x4 (exact f32 products and sums), bf16 calls 32 keys and
+// 16x16x32. Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that lane
+// (n = lane % 16, g = lane / 16) keeps query row n throughout: its maximum, its sum, its rescaling
+// factor, and keys 16 T + 4 g + r of score tile T, which are the second product's operand as they
+// stand. V's rows are read in the order of those keys, CW columns to a lane, one MFMA a column
+// (bf16: pairs of keys put together from two rows by byte permutes); columns come out as
+// 16 CW c + CW (4 g + r) + j in register r of accumulator c CW + j.
+// K of the next block is requested when this one's scores are formed, V when its output is: each is
+// on its way through the other's product, and two workgroups share a CU, so that one's prologue and
+// merge pass under the other's reads. The waves' states merge through LDS.
+constexpr int kRowWaves = 4;
 template <typename T, int D>
-__global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq_rows(SeqArgs a) {
-    constexpr int kRowWaves = row_waves<D>();
-    constexpr int NI = D / 16;  // loads of a lane per K block and head row
-    constexpr int NC = D / 64;  // and per V row
-    constexpr int NH = D / 32;  // loads of half a K (V) block
+__global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows(SeqArgs a) {
+    constexpr bool BF = sizeof(T) == 2;
+    constexpr int BK = BF ? 32 : 16;             // keys of a block
+    constexpr int NT = BK / 16;                  // score tiles of it
+    constexpr int EL = 16 / sizeof(T);           // elements of a load
+    constexpr int NI = D / (4 * EL);             // K loads of a lane to a tile
+    constexpr int CW = BF && D > 64 ? 8 : 4;     // columns of a V load
+    constexpr int NC = D / (16 * CW);            // V loads of a lane to a row
+    constexpr int NR = BF ? 8 : 4;               // V rows of a lane
+    constexpr int OS = D + 4;                    // row of the merge buffer
     constexpr int SLOTS = D > 256 ? 2 : 4;
-    __shared__ float s_o[SLOTS][D / 4 * kWave];
+    constexpr float kSlack = 8.0f;               // log2: how far scores may pass the running maximum
+    __shared__ __align__(16) float s_o[SLOTS * 16 * OS];  // (the query rows before)
     __shared__ float s_m[kRowWaves][16], s_l[kRowWaves][16];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -41,218 +55,273 @@ __global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq
     const Seq q = seq_of(a, sq);
     const int r0 = __builtin_amdgcn_readfirstlane(tile) * 16, rows = q.nq * a.gq, r1 = min(r0 + 16, rows) - 1;
     if (r0 >= rows) return;
-    const Range rg = tile_range(a, q, r0, r1, a.nsplit);
+    const Range rg = tile_range(a, q, r0, r1, a.chunk);
     if (split >= rg.used) return;
-    const int ks = rg.ks + split * rg.chunk, ke = min(rg.ke, ks + rg.chunk);
-    const int nblk = ke > ks ? (ke - ks + 15) / 16 : 0;
-    // the lane's query row and its range of keys [lo, hi]
+    const int ks = rg.ks + split * a.chunk, ke = rg.ke - ks > a.chunk ? ks + a.chunk : rg.ke;
+    const int nblk = ke > ks ? (ke - ks + BK - 1) / BK : 0;
+    // the lane's query row and its range of keys [lo, hi] (rows behind the last are the last once more)
     const int rr = min(r0 + n, r1), i = rr / a.gq, p = q.pos0 + i;
-    const bool valid = r0 + n <= r1 && p >= 0 && p < q.lim;
-    const int hi = valid ? p : -1;
+    const int hi = p >= 0 && p < q.lim ? p : -1;
     const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
     // the part of the keys that every row sees
     const int pf = q.pos0 + r0 / a.gq, pl = q.pos0 + r1 / a.gq;
-    const bool whole = r0 + 15 == r1 && pf >= 0 && pl < q.lim;
+    const bool whole = pf >= 0 && pl < q.lim;
     const int all_lo = a.window > 0 ? max(0, pl + 1 - a.window) : 0, all_hi = pf;
 
-    const T* const kbase = (const T*)a.kc + kvh * D + 4 * g;
-    const T* const vbase = (const T*)a.vc + kvh * D + 4 * n;
-    float* const s_q = &s_o[0][0] + 4 * lane;
+    u32x4* const s_q = reinterpret_cast<u32x4*>(s_o) + lane;
     {
-        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + 4 * g;
-        for (int j = wave; j < NI; j += kRowWaves) *reinterpret_cast<f32x4*>(s_q + 4 * kWave * j) = ld4(qrow + 16 * j);
+        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + EL * g;
+        const uint32_t flip = BF && !(a.softcap > 0.0f) && a.scale < 0.0f ? 0x80008000u : 0u;  // `unit` has no sign
+        for (int j = wave; j < NI; j += kRowWaves) s_q[kWave * j] = ld16(qrow + 4 * EL * j) ^ flip;
     }
-    __syncthreads();
-    acc4 o[NC * 4];
+    acc4 o[NC * CW];
 #pragma unroll
-    for (int j = 0; j < NC * 4; ++j) o[j] = acc4{};
+    for (int j = 0; j < NC * CW; ++j) o[j] = acc4{};
     float m = -INFINITY, l = 0.0f;
+    bool wild = false;  // infinite or NaN values were kept out of the product
 
-    f32x4 bx[NH], by[NH];
-    // The lane's key is n of a block: its row, -1 where there is none. Keys past the range take its last
-    // row (masked).
-    auto rows_of = [&](int blk) { return row_of(a, q, min(ks + 16 * blk + n, ke - 1)); };
-    auto load_k = [&](f32x4 (&r)[NH], int row, int half) {
-        const T* kp = kbase + (int64_t)max(row, 0) * a.kv_stride;
-#pragma unroll
-        for (int j = 0; j < NH; ++j) r[j] = ld4(kp + 16 * (NH * half + j));
+    // The lane's key is lane % BK of a block: its row, -1 where there is none (past the range, or on
+    // a page that is not in the cache).
+    auto rows_of = [&](int blk) {
+        const int key = ks + BK * blk + lane % BK, r = row_of(a, q, min(key, ke - 1));
+        return key < ke ? r : -1;
     };
-    auto load_v = [&](f32x4 (&r)[NH], int row, int half) {
+    const T* const kbase = (const T*)a.kc + kvh * D + EL * g;
+    const T* const vbase = (const T*)a.vc + kvh * D + CW * n;
+    u32x4 kk[NT][NI];
+    typedef uint32_t vload __attribute__((ext_vector_type(BF ? CW / 2 : 4)));
+    vload vv[NR][NC];
+    auto load_k = [&](int row) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const T* vp = vbase + (int64_t)max(__shfl(row, 4 * g + 2 * half + j), 0) * a.kv_stride;
+        for (int t = 0; t < NT; ++t) {
+            const T* kp = kbase + (int64_t)max(__shfl(row, 16 * t + n), 0) * a.kv_stride;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) r[NC * j + c] = ld4(vp + 64 * c);
+            for (int j = 0; j < NI; ++j) kk[t][j] = ld16(kp + 4 * EL * j);
         }
     };
-    int row = 0, row_next = 0;
-    if (wave < nblk) {
-        row = rows_of(wave);
-        load_k(bx, row, 0);
-    }
-    for (int blk = wave; blk < nblk; blk += kRowWaves) {
-        const int k0 = ks + 16 * blk;
-        row_next = rows_of(min(blk + kRowWaves, nblk - 1));
-        // scores: 16 products at a time into a fresh accumulator, these summed in two chains
-        acc4 st[2] = {acc4{}, acc4{}};
-        auto scores = [&](const f32x4 (&kr)[NH], int half) {
+    auto load_v = [&](int row) {
 #pragma unroll
-            for (int j = 0; j < NH; ++j) {
-                const f32x4 qv = *reinterpret_cast<const f32x4*>(s_q + 4 * kWave * (NH * half + j));
+        for (int e = 0; e < NR; ++e) {
+            const T* vp = vbase + (int64_t)max(__shfl(row, 16 * (e / 4) + 4 * g + e % 4), 0) * a.kv_stride;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) vv[e][c] = *reinterpret_cast<const vload*>(vp + 16 * CW * c);
+        }
+    };
+    // (past the last block, and in waves without one, row 0 of the cache is loaded: no load under a branch)
+    int row = wave < nblk ? rows_of(wave) : -1, next = wave + kRowWaves < nblk ? rows_of(wave + kRowWaves) : -1;
+    load_k(row);
+    load_v(row);
+    __syncthreads();  // the query rows
+    for (int blk = wave; blk < nblk; blk += kRowWaves) {
+        const int k0 = ks + BK * blk;
+        float x[4 * NT];
+        if constexpr (BF) {
+            acc4 s[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t] = acc4{};
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const bf16x8 qv = __builtin_bit_cast(bf16x8, s_q[kWave * j]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk[t][j]), qv, s[t], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4 * NT; ++e) {
+                x[e] = s[e / 4][e % 4];
+                if (a.softcap > 0.0f) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e] * a.scale, a.softcap, a.inv_cap));
+            }
+        } else {
+            // 16 products at a time into a fresh accumulator, these summed in two chains: one chain over the
+            // whole row is two to three times as far from the exact dot product
+            acc4 st[2] = {acc4{}, acc4{}};
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const f32x4 qv = __builtin_bit_cast(f32x4, s_q[kWave * j]), kv = __builtin_bit_cast(f32x4, kk[0][j]);
                 acc4 c = acc4{};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[j][e], qv[e], c, 0, 0, 0);
+                for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[e], c, 0, 0, 0);
                 st[j & 1] += c;
             }
-        };
-        load_k(by, row, 1);
-        scores(bx, 0);
-        load_v(bx, row, 0);
-        scores(by, 1);
-        load_v(by, row, 1);
-        // (row -1: keys 4 g + r of the block whose page is not in the cache)
-        const bool gap = __any(row < 0);
-        const bool edge = gap || !(whole && k0 >= all_lo && k0 + 15 <= all_hi);  // uniform
-        float s[4], mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float v = (st[0][r] + st[1][r]) * a.scale;
-            if (a.softcap > 0.0f) v = a.softcap * tanh_fast(div_by_uniform(v, a.softcap, a.inv_cap));
-            const int key = k0 + 4 * g + r;
-            const bool there = !gap || __shfl(row, 4 * g + r) >= 0;
-            s[r] = key >= lo && key <= hi && key < ke && there ? v : -INFINITY;
-            mx = fmaxf(mx, s[r]);
+            for (int e = 0; e < 4; ++e) {
+                x[e] = (st[0][e] + st[1][e]) * a.scale;
+                if (a.softcap > 0.0f) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+            }
         }
+        const int row_v = row;
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay behind the last use of their registers
+        load_k(next);
+        row = next;
+        if (blk + 2 * kRowWaves < nblk) next = rows_of(blk + 2 * kRowWaves);
+        else next = -1;
+        __builtin_amdgcn_sched_barrier(0);
+        const bool none = __any(row_v < 0);
+        const bool edge = none || !(whole && k0 >= all_lo && k0 + BK - 1 <= all_hi);  // uniform
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 4 * NT; ++e) {
+                const int kb = 16 * (e / 4) + 4 * g + e % 4, key = k0 + kb;
+                const bool there = __shfl(row_v, kb) >= 0;
+                x[e] = key >= lo && key <= hi && there ? x[e] : -INFINITY;
+            }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int e = 1; e < 4 * NT; ++e) mx = fmaxf(mx, x[e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.0f : mn;
-        const float c = exp2f((m - ms) * kLog2e);
-        float pr[4], ps = 0.0f;
+        if (__any(!((mx - m) * a.unit <= kSlack))) {
+            const float mn = fmaxf(m, mx);
+            const float c = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * a.unit);
+            m = mn;
+            l *= c;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            pr[r] = exp2f((s[r] - ms) * kLog2e);
-            ps += pr[r];
+            for (int j = 0; j < NC * CW; ++j) o[j] *= c;
         }
-        l = l * c + ps;
-        m = mn;
-        if (!__all(c == 1.0f)) {  // rows 4 g + r of the output accumulators
+        const float ms = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float cr = __shfl(c, 4 * g + r);
-#pragma unroll
-                for (int j = 0; j < NC * 4; ++j) o[j][r] *= cr;
-            }
+        for (int e = 0; e < 4 * NT; ++e) {
+            x[e] = __builtin_amdgcn_exp2f((x[e] - ms) * a.unit);
+            l += x[e];
         }
         if (edge) {
-            float z = 0.0f;  // NaN if a V value is infinite or NaN
+            // A weight of 0 must not carry an infinite or NaN value to a row that does not see it: such
+            // values stay out, and go to the rows that see them at the end.
+            bool bad = false;
 #pragma unroll
-            for (int j = 0; j < NH; ++j)
+            for (int e = 0; e < NR; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z += bx[j][e] * 0.0f + by[j][e] * 0.0f;
-            if (__any(!(z == 0.0f))) {
-                // Some of the query rows may see such a row and others not: 0 * V would reach the others,
-                // so each takes just the keys it sees, and the products below add zeros.
-#pragma unroll 1
-                for (int k = 0; k < 16; ++k) {
-                    const int rk = __shfl(row, k);
-                    if (k0 + k >= ke || rk < 0) continue;  // uniform
-                    const T* vp = vbase + (int64_t)rk * a.kv_stride;
+                for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float pk = __shfl(k & 2 ? (k & 1 ? pr[3] : pr[2]) : (k & 1 ? pr[1] : pr[0]),
-                                                4 * g + r + 16 * (k >> 2));
-                        const int rlo = __shfl(lo, 4 * g + r), rhi = __shfl(hi, 4 * g + r);
-                        if (k0 + k >= rlo && k0 + k <= rhi) {
-#pragma unroll
-                            for (int cc = 0; cc < NC; ++cc) {
-                                const f32x4 v = ld4(vp + 64 * cc);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[cc * 4 + e][r] = fmaf(pk, v[e], o[cc * 4 + e][r]);
-                            }
+                    for (int w = 0; w < (int)(sizeof(vload) / 4); ++w) {
+                        uint32_t v = vv[e][c][w];
+                        if constexpr (BF) {
+                            const bool b0 = (v & 0x7f80u) == 0x7f80u, b1 = (v & 0x7f800000u) == 0x7f800000u;
+                            bad |= b0 || b1;
+                            v &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu);
+                        } else {
+                            const bool b = (v & 0x7f800000u) == 0x7f800000u;
+                            bad |= b;
+                            v = b ? 0u : v;
                         }
+                        vv[e][c][w] = v;
                     }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) pr[r] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < NH; ++j) bx[j] = by[j] = f32x4{};
-            }
+            wild |= __any(bad) != 0;
         }
-        auto pv = [&](const f32x4 (&v)[NH], int half) {
+        if constexpr (BF) {
+            u32x4 pw;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int e = 0; e < 4; ++e) pw[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+            const bf16x8 pv = __builtin_bit_cast(bf16x8, pw);
 #pragma unroll
-                for (int cc = 0; cc < NC; ++cc)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[cc * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pr[2 * half + j], v[NC * j + cc][e],
-                                                                             o[cc * 4 + e], 0, 0, 0);
-        };
-        pv(bx, 0);
-        load_k(bx, row_next, 0);
-        pv(by, 1);
-        row = row_next;
+                for (int w = 0; w < CW / 2; ++w) {
+                    u32x4 v0, v1;  // columns 2 w and 2 w + 1 of the lane's eight keys
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v0[e] = __builtin_amdgcn_perm(vv[2 * e + 1][c][w], vv[2 * e][c][w], 0x05040100u);
+                        v1[e] = __builtin_amdgcn_perm(vv[2 * e + 1][c][w], vv[2 * e][c][w], 0x07060302u);
+                    }
+                    acc4 &o0 = o[c * CW + 2 * w], &o1 = o[c * CW + 2 * w + 1];
+                    o0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v0), pv, o0, 0, 0, 0);
+                    o1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v1), pv, o1, 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        o[c * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vv[e][c][j]), x[e], o[c * 4 + j], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(row);
+    }
+    if (wild) {
+        // What a row sees of the values kept out: whatever its weight, the value itself (which changes nothing
+        // where it went in).
+#pragma unroll 1
+        for (int k = 0; k < nblk * BK; ++k) {
+            const int key = ks + k;
+            if (k / BK % kRowWaves != wave || key >= ke) continue;
+            const int r = row_of(a, q, key);
+            if (r < 0 || key < lo || key > hi) continue;
+            const T* const vp = (const T*)a.vc + (int64_t)r * a.kv_stride + kvh * D + 4 * CW * g;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < CW; j += 4) {
+                        const f32x4 v = ld4(vp + 16 * CW * c + CW * e + j);
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) o[c * CW + j + z][e] += fabsf(v[z]) < INFINITY ? 0.0f : v[z];
+                    }
+        }
     }
 
     // Merge: each wave's state scaled to the common maximum, SLOTS waves at a time into the slots, which
     // every thread then adds in slot order.
-    __syncthreads();  // every wave is done with the query rows
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if (l == 0.0f) {  // no key: zeros, whatever weights of 0 made of the values
+#pragma unroll
+        for (int j = 0; j < NC * CW; ++j) o[j] = acc4{};
+    }
     if (g == 0) {
         s_m[wave][n] = m;
         s_l[wave][n] = l;
     }
-    __syncthreads();
+    __syncthreads();  // and every wave is done with the query rows
+    {
+        float M = s_m[0][n];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int rw = 4 * g + r;
-        float M = s_m[0][rw];
+        for (int w = 1; w < kRowWaves; ++w) M = fmaxf(M, s_m[w][n]);
+        const float f = __builtin_amdgcn_exp2f((m - (M == -INFINITY ? 0.0f : M)) * a.unit);
 #pragma unroll
-        for (int w = 1; w < kRowWaves; ++w) M = fmaxf(M, s_m[w][rw]);
-        const float f = exp2f((s_m[wave][rw] - (M == -INFINITY ? 0.0f : M)) * kLog2e);
-#pragma unroll
-        for (int j = 0; j < NC * 4; ++j) o[j][r] *= f;
+        for (int j = 0; j < NC * CW; ++j) o[j] *= f;
     }
-    float* const slot = s_o[wave % SLOTS] + lane;
+    float* const slot = s_o + (wave % SLOTS * 16 + n) * OS + 4 * CW * g;
 #pragma unroll
     for (int w0 = 0; w0 < kRowWaves; w0 += SLOTS) {
-        if (wave >= w0 && wave < w0 + SLOTS) {
+        if (wave >= w0 && wave < w0 + SLOTS && r0 + n <= r1) {
 #pragma unroll
-            for (int j = 0; j < NC * 4; ++j)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = (j * 4 + r) * kWave;
-                    slot[at] = w0 == 0 ? o[j][r] : slot[at] + o[j][r];
-                }
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < CW; j += 4) {
+                        f32x4* const at = reinterpret_cast<f32x4*>(slot + 16 * CW * c + CW * e + j);
+                        f32x4 v{o[c * CW + j][e], o[c * CW + j + 1][e], o[c * CW + j + 2][e], o[c * CW + j + 3][e]};
+                        if (w0 > 0) v += *at;
+                        *at = v;
+                    }
         }
         __syncthreads();
     }
-    // row = 4 g + r, columns 64 c + 4 n + e: four of a row per thread
     for (int t = threadIdx.x; t < 16 * D / 4; t += kRowWaves * kWave) {
-        const int rw = t / (D / 4), col = t % (D / 4), c = col / 16, nn = col % 16;
-        if (r0 + rw > r1) continue;
+        const int rw = t / (D / 4), col = t % (D / 4) * 4;
+        if (r0 + rw > r1) break;
         const int64_t tok = q.tok0 + (r0 + rw) / a.gq, h = kvh * a.gq + (r0 + rw) % a.gq;
         float M = s_m[0][rw], L = 0.0f;
 #pragma unroll
         for (int w = 1; w < kRowWaves; ++w) M = fmaxf(M, s_m[w][rw]);
 #pragma unroll
-        for (int w = 0; w < kRowWaves; ++w) L += s_l[w][rw] * exp2f((s_m[w][rw] - (M == -INFINITY ? 0.0f : M)) * kLog2e);
-        f32x4 v;
+        for (int w = 0; w < kRowWaves; ++w)
+            L += s_l[w][rw] * __builtin_amdgcn_exp2f((s_m[w][rw] - (M == -INFINITY ? 0.0f : M)) * a.unit);
+        f32x4 v{};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x = 0.0f;
-#pragma unroll
-            for (int w = 0; w < SLOTS; ++w) x += s_o[w][((c * 4 + e) * 4 + (rw & 3)) * kWave + 16 * (rw >> 2) + nn];
-            v[e] = x;
-        }
+        for (int w = 0; w < SLOTS; ++w) v += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + rw) * OS + col);
         if (rg.used == 1) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = L == 0.0f ? 0.0f : v[e] / L;  // (no key: zeros)
-            st4((T*)a.out + (tok * a.nh + h) * D + 4 * col, v);
+            st4((T*)a.out + (tok * a.nh + h) * D + col, v);
         } else {
             const int64_t part = (tok * a.nh + h) * a.nparts + split;
-            st4(a.ws + part * D + 4 * col, v);
+            st4(a.ws + part * D + col, v);
             if (col == 0) {
                 float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
                 ml[0] = M;
@@ -262,18 +331,35 @@ __global__ __launch_bounds__(row_waves<D>() * kWave, D > 256 ? 1 : 2) void k_seq
     }
 }
 
-// Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s, a wave
-// each. The row's splits are those of the tile that formed them.
+// Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s, a workgroup
+// each, wave w the splits w, w + 4, ... The row's splits are those of the tile that formed them. The
+// maxima and the first sums are requested before their number is known (slots behind it hold
+// anything: they are dropped, not weighted by 0), which leaves one round trip to memory behind the
+// sequence's own.
 constexpr int kMaxSplits = 256;
 constexpr int kJoinWaves = 4;
 template <typename T, int D>
 __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     constexpr int E = D / 64;  // columns of a lane
     constexpr int PER = kMaxSplits / kWave;
-    const int lane = threadIdx.x & 63;
-    const int64_t th = (int64_t)blockIdx.x * kJoinWaves + (threadIdx.x >> 6);
-    if (th >= (int64_t)a.n_tokens * a.nh) return;
-    const int tok = __builtin_amdgcn_readfirstlane((int)(th / a.nh)), h = (int)(th % a.nh);
+    constexpr int PRE = 4;
+    typedef float Cols __attribute__((ext_vector_type(E)));
+    __shared__ float s_part[kJoinWaves][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t th = blockIdx.x, part = th * a.nparts;
+    const int tok = (int)(th / a.nh), h = (int)(th % a.nh);
+    const float* const ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
+    const float* const sums = a.ws + part * D + E * lane;
+    float mv[PER], lv[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int sp = min(lane + j * kWave, a.nparts - 1);
+        mv[j] = ml[2 * sp];
+        lv[j] = ml[2 * sp + 1];
+    }
+    Cols pre[PRE];
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) pre[k] = *reinterpret_cast<const Cols*>(sums + (int64_t)min(wave + k * kJoinWaves, a.nparts - 1) * D);
     int sq = tok;
     if (a.cu) {
         // the last sequence that begins at or before the token
@@ -292,46 +378,44 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     const int rows = q.nq * a.gq;
     const bool few = rows <= a.few_rows;
     const int R = few ? 16 : a.tile_rows;
-    const float unit = few ? kLog2e : a.unit;
     const int r = (tok - q.tok0) * a.gq + h % a.gq, r0 = r / R * R, r1 = min(r0 + R, rows) - 1;
-    const Range rg = tile_range(a, q, r0, r1, few ? a.nsplit : a.tile_split);
-    if (rg.used == 1) return;
-    const int64_t part = th * a.nparts;
-    const float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
-    float mv[PER], lv[PER], M = -INFINITY;
+    const int used = tile_range(a, q, r0, r1, few ? a.chunk : a.tile_chunk).used;
+    if (used == 1) return;
+    float M = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int sp = lane + j * kWave;
-        mv[j] = sp < rg.used ? ml[2 * sp] : -INFINITY;
-        lv[j] = sp < rg.used ? ml[2 * sp + 1] : 0.0f;
-        M = fmaxf(M, mv[j]);
-    }
+    for (int j = 0; j < PER; ++j) M = fmaxf(M, lane + j * kWave < used ? mv[j] : -INFINITY);
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
     float L = 0.0f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        mv[j] = exp2f((mv[j] - (M == -INFINITY ? 0.0f : M)) * unit);
-        L = fmaf(lv[j], mv[j], L);
+        mv[j] = __builtin_amdgcn_exp2f((mv[j] - (M == -INFINITY ? 0.0f : M)) * a.unit);
+        if (lane + j * kWave < used) L = fmaf(lv[j], mv[j], L);
     }
     L = group_sum<kWave>(L);
-    float acc[E] = {};
+    Cols acc = Cols{};
+    // the weight of split sp
+    auto weight = [&](int sp) {
+        float c = mv[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int end = min(rg.used - j * kWave, kWave);
-        for (int sp = 0; sp < end; ++sp) {
-            const float c = __shfl(mv[j], sp);
-            const float* w = a.ws + (part + j * kWave + sp) * D + E * lane;
+        for (int j = 1; j < PER; ++j) c = sp / kWave == j ? mv[j] : c;
+        return __shfl(c, sp % kWave);
+    };
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(w[e], c, acc[e]);
-        }
+    for (int k = 0; k < PRE; ++k) {
+        const int sp = wave + k * kJoinWaves;
+        if (sp < used) acc += pre[k] * weight(sp);
     }
-    T* out = (T*)a.out + th * D + E * lane;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float v = L == 0.0f ? 0.0f : acc[e] / L;
-        if constexpr (sizeof(T) == 4) out[e] = v;
-        else out[e] = (T)(pack_bf16x2(v, 0.0f) & 0xffffu);
+#pragma unroll 4
+    for (int sp = wave + PRE * kJoinWaves; sp < used; sp += kJoinWaves)
+        acc += *reinterpret_cast<const Cols*>(sums + (int64_t)sp * D) * weight(sp);
+    *reinterpret_cast<Cols*>(&s_part[wave][E * lane]) = acc;
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += kJoinWaves * kWave) {
+        const float t = (s_part[0][c] + s_part[1][c]) + (s_part[2][c] + s_part[3][c]);
+        const float v = L == 0.0f ? 0.0f : t / L;
+        if constexpr (sizeof(T) == 4) ((T*)a.out)[th * D + c] = v;
+        else ((T*)a.out)[th * D + c] = (T)(pack_bf16x2(v, 0.0f) & 0xffffu);
     }
 }
 
@@ -340,21 +424,29 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
 // Which kernels a call takes, and the splits of each one's ranges. k_seq_tile takes bf16 calls'
 // sequences of more than 16 query rows; a call whose sequences all have that few (a token each), or
 // surely more (a prompt, one chunk), launches one kernel only.
-// Splits: as many as bring the launch to about 512 workgroups (256 of k_seq_tile), none shorter than 128
-// (256) keys of the longest possible range.
+// Splits have one size in a call, whatever the sequences' lengths, which evens out the workgroups of a ragged
+// batch. k_seq_rows's: half a megabyte of K and V, less where that leaves under 1024 workgroups;
+// k_seq_tile's: where there are under 512 workgroups, down to 256 keys.
 static void choose(SeqArgs& a, int dtype) {
     a.gq = a.nh / a.nkv;
     a.tile_rows = tile_rows_of(a.D);
     const bool single = a.table && !a.cu;  // a token each
     if (dtype != HIP_BRIDGE_BF16 || (int64_t)a.n_tokens * a.gq <= 16 || (single && a.gq <= 16)) a.few_rows = INT32_MAX;
     else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : 16;
-    auto splits = [&](int R, int wgs, int least) {
-        const int64_t len = a.window > 0 ? std::min<int64_t>((int64_t)a.window + (R - 1) / a.gq, a.max_len) : a.max_len;
-        const int64_t want = cdiv(wgs, std::max<int64_t>(most_tiles(a, R) * a.nkv, 1));
-        return (int)std::max<int64_t>(1, std::min<int64_t>({want, cdiv(len, least), (int64_t)kMaxSplits}));
+    const int64_t es = dtype == HIP_BRIDGE_F32 ? 4 : 2;
+    auto splits = [&](int R, int64_t wgs, int64_t least, int64_t most, int& chunk) {
+        const int64_t len = most_keys(a, R), groups = most_tiles(a, R) * a.nkv;
+        int64_t keys = std::min(most, cdiv(cdiv(len * groups, wgs), 64) * 64);
+        keys = std::max({keys, least, cdiv(cdiv(len, kMaxSplits), 64) * 64});
+        chunk = (int)std::min<int64_t>(keys, INT32_MAX);
+        return (int)std::max<int64_t>(cdiv(len, keys), 1);
     };
-    a.nsplit = a.few_rows > 0 ? splits(16, 512, 128) : 1;
-    a.tile_split = a.few_rows < INT32_MAX ? splits(a.tile_rows, 256, 256) : 1;
+    a.nsplit = a.tile_split = 1;
+    a.chunk = a.tile_chunk = INT32_MAX;
+    if (a.few_rows > 0) a.nsplit = splits(16, 1024, 64, (1 << 18) / (a.D * es), a.chunk);
+    if (a.few_rows < INT32_MAX) {
+        if (most_tiles(a, a.tile_rows) * a.nkv < 256) a.tile_split = splits(a.tile_rows, 512, 256, INT32_MAX, a.tile_chunk);
+    }
     a.nparts = std::max(a.nsplit, a.tile_split);
 }
 static size_t split_bytes(const SeqArgs& a) {
@@ -379,12 +471,12 @@ template <typename T, int D>
 static void launch_rows(const SeqArgs& a, hipStream_t s) {
     if (a.few_rows > 0) {
         const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
-        k_seq_rows<T, D><<<(unsigned)grid, row_waves<D>() * kWave, 0, s>>>(a);
+        k_seq_rows<T, D><<<(unsigned)grid, kRowWaves * kWave, 0, s>>>(a);
     }
     if (a.few_rows < INT32_MAX) launch_tiles(a, s);
     if (a.nparts > 1) {
         const int64_t th = (int64_t)a.n_tokens * a.nh;
-        k_seq_join<T, D><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
+        k_seq_join<T, D><<<(unsigned)th, kJoinWaves * kWave, 0, s>>>(a);
     }
     check_launch();
 }
@@ -411,11 +503,14 @@ static void launch_seqs(int dtype, SeqArgs& a, void* ws, size_t ws_bytes, hipStr
         return;
     }
     choose(a, dtype);
-    if (a.nparts > 1 && (!ws || !aligned16(ws) || split_bytes(a) > ws_bytes)) a.nsplit = a.tile_split = a.nparts = 1;
+    if (a.nparts > 1 && (!ws || !aligned16(ws) || split_bytes(a) > ws_bytes)) {
+        a.nsplit = a.tile_split = a.nparts = 1;
+        a.chunk = a.tile_chunk = INT32_MAX;
+    }
     a.ws = (float*)ws;
     a.inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     // (never 0: a masked score of -inf times it stays -inf)
-    a.unit = std::max(a.softcap > 0.0f ? kLog2e : kLog2e * std::fabs(a.scale), 1e-30f);
+    a.unit = dtype == HIP_BRIDGE_F32 || a.softcap > 0.0f ? kLog2e : std::max(kLog2e * std::fabs(a.scale), 1e-30f);
     if (most_tiles(a, 16) * a.nkv * a.nparts > INT32_MAX) {
         set_error(HIP_BRIDGE_EUNSUPPORTED);
         return;

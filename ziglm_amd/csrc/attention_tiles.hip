@@ -20,7 +20,6 @@
 
 namespace zl {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
@@ -68,9 +67,11 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     constexpr int NC = KB * CR / TH;     // of a tile, to a thread
     constexpr int RS = TH / CR;          // rows between a thread's chunks
     constexpr float kSlack = 8.0f;       // log2
-    static_assert(KB * CR % TH == 0 && TH % CR == 0, "chunks of a tile");
-    __shared__ __align__(16) uint8_t s_k[2][KB * D * 2], s_v[2][KB * D * 2];
-    __shared__ uint32_t s_gap[3][KB / 32], s_bad[3];  // keys without a row; V has an infinite or NaN value
+    static_assert(KB * CR % TH == 0 && TH % CR == 0 && RS % 8 == 0, "chunks of a tile");
+    constexpr int TB = KB * D * 2;       // bytes of a tile of K or V
+    __shared__ __align__(16) uint8_t s_kv[2][2][TB];  // [buffer][K, V]
+    __shared__ uint32_t s_gap[3][KB / 32];  // keys without a row
+    __shared__ int s_wild;                  // infinite or NaN values were kept out of LDS
     const int tid = threadIdx.x, lane = tid & 63, n = lane % M, h = lane / M;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = (int)blockIdx.x;
@@ -86,18 +87,18 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     const int r0 = ((rows + NW * M - 1) / (NW * M) - 1 - __builtin_amdgcn_readfirstlane(tile)) * (NW * M);
     if (r0 < 0 || r0 >= rows) return;
     const int r1 = min(r0 + NW * M, rows) - 1;
-    const Range rg = tile_range(a, q, r0, r1, a.tile_split);
+    const Range rg = tile_range(a, q, r0, r1, a.tile_chunk);
     if (split >= rg.used) return;
-    const int ks = rg.ks + split * rg.chunk, ke = min(rg.ke, ks + rg.chunk);
+    const int ks = rg.ks + split * a.tile_chunk, ke = rg.ke - ks > a.tile_chunk ? ks + a.tile_chunk : rg.ke;
     const int ntile = ke > ks ? (ke - ks + KB - 1) / KB : 0;
 
     // the lane's query row and its keys [lo, hi], and what all of the wave's rows see
     const int w0 = r0 + wave * M, w1 = min(w0 + M - 1, r1);
     const int rr = min(w0 + n, r1), i = rr / a.gq, p = q.pos0 + i;
-    const int hi = w0 + n <= r1 && p >= 0 && p < q.lim ? p : -1;
+    const int hi = p >= 0 && p < q.lim ? p : -1;  // (rows behind the last are the last once more)
     const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
     const int pf = q.pos0 + w0 / a.gq, pl = q.pos0 + max(w1, 0) / a.gq;
-    const bool whole = w0 + M - 1 <= r1 && pf >= 0 && pl < q.lim;
+    const bool whole = pf >= 0 && pl < q.lim;
     const int any_lo = a.window > 0 ? max(0, pf + 1 - a.window) : 0, all_lo = a.window > 0 ? max(0, pl + 1 - a.window) : 0;
     const int any_hi = w0 <= r1 ? min(pl, q.lim - 1) : -1, all_hi = pf;
     // and of the workgroup's: tiles outside have keys that some rows do not see
@@ -155,24 +156,43 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             }
         }
         if (k0 < wg_lo || k0 + KB - 1 > wg_hi) {
+            // Some rows do not see all of the tile's keys: infinite and NaN values, which weights of 0 would
+            // carry to them, stay out of LDS, and go to the rows that see them at the end.
             bool bad = false;
 #pragma unroll
             for (int j = 0; j < NC; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     bad |= (bv[j][e] & 0x7f80u) == 0x7f80u || (bv[j][e] & 0x7f800000u) == 0x7f800000u;
-            if (__any(bad) && lane == 0) s_bad[f] = 1;
+            if (__any(bad)) {
+                if (lane == 0) s_wild = 1;
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if ((bv[j][e] & 0x7f80u) == 0x7f80u) bv[j][e] &= 0xffff0000u;
+                        if ((bv[j][e] & 0x7f800000u) == 0x7f800000u) bv[j][e] &= 0xffffu;
+                    }
+            }
         }
+        uint8_t* const kd = &s_kv[buf][0][sr * D * 2 + ((sc ^ (sr & 7)) << 4)];
+        uint8_t* const vd = &s_kv[buf][1][sr * D * 2 + ((sc ^ ((sr & 3) << 1)) << 4)];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const int r = sr + j * RS;
-            *reinterpret_cast<u32x4*>(&s_k[buf][r * D * 2 + ((sc ^ (r & 7)) << 4)]) = bk[j];
-            *reinterpret_cast<u32x4*>(&s_v[buf][r * D * 2 + ((sc ^ ((r & 3) << 1)) << 4)]) = bv[j];
+            *reinterpret_cast<u32x4*>(kd + j * RS * D * 2) = bk[j];
+            *reinterpret_cast<u32x4*>(vd + j * RS * D * 2) = bv[j];
         }
     };
+    // The lane's LDS addresses: the swizzle is an exclusive or of the low three bits of a chunk's index,
+    // so the operands lie at few bases and offsets that are known here. K: chunk j G + h of row T M + n;
+    // V: chunk b M / 8 + vc (+ 8 bytes) of row u US + 4 h + lane % 16 / 4.
+    constexpr int KBASES = 8 / G, VBASES = 64 / M;
+    const int li = lane & 15;
+    const int ky = h ^ (n & 7), vy = ((M == 32 ? 2 * (lane >> 4 & 1) : 0) + ((li & 3) >> 1)) ^ (li >> 2 << 1);
+    const int kn = n * D * 2, vn = (4 * h + (li >> 2)) * D * 2 + (li & 1) * 8;
 
+    if (tid == 0) s_wild = 0;
     if (tid < 3) {
-        s_bad[tid] = 0;
 #pragma unroll
         for (int e = 0; e < KB / 32; ++e) s_gap[tid][e] = 0;
     }
@@ -198,12 +218,14 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             if (t + 2 < ntile) find_rows(t + 2);
         }
         if (tid == 0) {  // the flags that tile t - 1 had are tile t + 2's
-            s_bad[(t + 2) % 3] = 0;
 #pragma unroll
             for (int e = 0; e < KB / 32; ++e) s_gap[(t + 2) % 3][e] = 0;
         }
         if (k0 <= any_hi && k0 + KB > any_lo) {  // (uniform: some row of the wave sees some key)
             // scores
+            const uint8_t* kb[KBASES];
+#pragma unroll
+            for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[buf][0][kn + ((c * G ^ ky) << 4)];
             Acc s[NT];
 #pragma unroll
             for (int T = 0; T < NT; ++T) s[T] = Acc{};
@@ -211,8 +233,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
-                    const int r = T * M + n;
-                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(&s_k[buf][r * D * 2 + (((j * G + h) ^ (r & 7)) << 4)]);
+                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb[j % KBASES] + T * M * D * 2 + (j / KBASES << 7));
                     s[T] = Mfma<M>::run(kv, qv[j], s[T]);
                 }
             float x[NT * SR];
@@ -253,46 +274,23 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
                 ps += x[e];
             }
             l += ps;
-            if (__builtin_amdgcn_readfirstlane(s_bad[f])) {
-                // Some rows see an infinite or NaN value and others do not: 0 * V would reach the others, so
-                // each takes just the keys it sees.
-#pragma unroll 1
-                for (int k = 0; k < KB; ++k) {
-                    float pk = 0.0f;
+            // output: MFMA t takes key groups 2 t and 2 t + 1
+            const uint8_t* vb[VBASES];
 #pragma unroll
-                    for (int e = 0; e < NT * SR; ++e)
-                        if (e / 4 == k / US && e % 4 == k % 4) pk = x[e];
-                    pk = __shfl(pk, n + M * (k % US / 4));
-                    if (k0 + k < lo || k0 + k > hi || (s_gap[f][k / 32] >> (k % 32) & 1)) continue;
+            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[buf][1][vn + ((c * (M / 8) ^ vy) << 4)];
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+            for (int u = 0; u < NU; u += 2) {
+                u32x4 pw;
 #pragma unroll
-                        for (int e = 0; e < SR; ++e) {
-                            const int d = b * M + e / 4 * 8 + 4 * h + e % 4;
-                            const uint16_t v = *reinterpret_cast<const uint16_t*>(
-                                &s_v[buf][k * D * 2 + (((d / 8) ^ ((k & 3) << 1)) << 4) + d % 8 * 2]);
-                            o[b][e] = fmaf(pk, __uint_as_float((uint32_t)v << 16), o[b][e]);
-                        }
-                }
-            } else {
-                // output: MFMA t takes key groups 2 t and 2 t + 1
-                const int li = lane & 15, gl = lane >> 4;
-                const int c0 = (M == 32 ? 2 * (gl & 1) : 0) + ((li & 3) >> 1), sw = li >> 2 << 1;
-                const uint8_t* const vrow = &s_v[buf][(4 * h + (li >> 2)) * D * 2 + (li & 1) * 8];
+                for (int e = 0; e < 4; ++e) pw[e] = pack_bf16x2(x[4 * u + 2 * e], x[4 * u + 2 * e + 1]);
+                const bf16x8 pv = __builtin_bit_cast(bf16x8, pw);
 #pragma unroll
-                for (int u = 0; u < NU; u += 2) {
-                    u32x4 pw;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) pw[e] = pack_bf16x2(x[4 * u + 2 * e], x[4 * u + 2 * e + 1]);
-                    const bf16x8 pv = __builtin_bit_cast(bf16x8, pw);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const int at = ((b * (M / 8) & ~7) | ((b * (M / 8) & 7) ^ c0 ^ sw)) << 4;
-                        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vrow + u * US * D * 2 + at));
-                        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vrow + (u + 1) * US * D * 2 + at));
-                        const bf16x8 vv = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[b] = Mfma<M>::run(vv, pv, o[b]);
-                    }
+                for (int b = 0; b < NB; ++b) {
+                    const uint8_t* const at = vb[b % VBASES] + (b / VBASES << 7);
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + u * US * D * 2));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (u + 1) * US * D * 2));
+                    const bf16x8 vv = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[b] = Mfma<M>::run(vv, pv, o[b]);
                 }
             }
         }
@@ -302,9 +300,33 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
 
     l = over_row<M>(l, [](float u, float v) { return u + v; });
     if (w0 + n > r1) return;
+    if (s_wild) {
+        // What a row sees of the values kept out: whatever its weight, the value itself.
+#pragma unroll 1
+        for (int k = ks; k < ke; ++k) {
+            const int k0 = ks + (k - ks) / KB * KB;
+            if (k0 >= wg_lo && k0 + KB - 1 <= wg_hi) continue;  // (uniform: the tile went whole)
+            const int r = row_of(a, q, k);
+            if (r < 0 || k < lo || k > hi) continue;
+            const uint16_t* const vp = (const uint16_t*)a.vc + (int64_t)r * a.kv_stride + kvh * D + 4 * h;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < SR; e += 4) {
+                    const f32x4 v = ld4(vp + b * M + 2 * e);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[b][e + c] += fabsf(v[c]) < INFINITY ? 0.0f : v[c];
+                }
+        }
+    }
+    if (l == 0.0f) {  // no key: zeros, whatever weights of 0 made of the values
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] = Acc{};
+        l = 1.0f;
+    }
     const int64_t th = (int64_t)(q.tok0 + i) * a.nh + kvh * a.gq + rr % a.gq;
     if (rg.used == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = 1.0f / l;
         uint16_t* out = (uint16_t*)a.out + th * D + 4 * h;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -333,12 +355,20 @@ static void launch(const SeqArgs& a, hipStream_t s) {
     else k_seq_tile<D, M, NW, KB, WPE, false><<<grid, NW * kWave, 0, s>>>(a);
 }
 
-int tile_rows_of(int D) { return D <= 128 ? 256 : D == 256 ? 128 : 128; }
+#ifndef ZL_T256
+#define ZL_T256 256, 16, 8, 32, 2
+#define ZL_R256 128
+#endif
+#ifndef ZL_T128
+#define ZL_T128 128, 32, 8, 64, 2
+#define ZL_R128 256
+#endif
+int tile_rows_of(int D) { return D <= 64 ? 256 : D == 128 ? ZL_R128 : D == 256 ? ZL_R256 : 128; }
 
 void launch_tiles(const SeqArgs& a, hipStream_t s) {
     if (a.D == 64) launch<64, 32, 8, 64, 2>(a, s);
-    else if (a.D == 128) launch<128, 32, 8, 64, 2>(a, s);
-    else if (a.D == 256) launch<256, 32, 4, 64, 1>(a, s);
+    else if (a.D == 128) launch<ZL_T128>(a, s);
+    else if (a.D == 256) launch<ZL_T256>(a, s);
     else launch<512, 16, 8, 32, 2>(a, s);
 }
 
