@@ -32,6 +32,7 @@ struct SeqArgs {
     int chunk, tile_chunk;           // keys of a split
     int tile_rows;         // query rows of a workgroup of k_seq_tile
     float scale, softcap, inv_cap;
+    float cap_in;          // 2 log2(e) scale / softcap
     float unit;            // of running maxima: log2(e); bf16: log2(e) * |scale|, or log2(e) where soft-capped
 };
 
@@ -127,6 +128,13 @@ inline int64_t most_keys(const SeqArgs& a, int R) {
     return a.window > 0 ? std::min<int64_t>((int64_t)a.window + cdiv(R - 1, a.gq), a.max_len) : a.max_len;
 }
 
+// Soft-capped score of a bf16 call: cap * tanh(z) = cap - 2 cap / (exp(2 z) + 1), z = x * scale / cap. The
+// difference of nearly equal terms near 0 is off by 2^-23 cap, far inside the rounding of the weights
+// (2^-8); f32 calls take the form that is exact to the last places there too.
+__device__ __forceinline__ float cap_bf16(const SeqArgs& a, float x) {
+    return fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.cap_in) + 1.0f), -2.0f * a.softcap, a.softcap);
+}
+
 // 4 consecutive elements as f32
 __device__ __forceinline__ f32x4 ld4(const float* p) { return ldf4(p); }
 __device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
@@ -142,8 +150,8 @@ __device__ __forceinline__ void st4(uint16_t* p, const f32x4& v) {
 inline int64_t most_tiles(const SeqArgs& a, int R) {
     return std::min<int64_t>((int64_t)a.n_tokens * a.gq / R + a.n_seqs, (int64_t)a.n_tokens * cdiv(a.gq, R));
 }
-// k_seq_tile (attention_tiles.hip): query rows of a workgroup for head size D, and the launch.
-int tile_rows_of(int D);
-void launch_tiles(const SeqArgs& a, hipStream_t s);
+// k_seq_tile (attention_tiles.hip): query rows of a workgroup for a type and head size, and the launch.
+int tile_rows_of(int dtype, int D, bool small);
+void launch_tiles(int dtype, const SeqArgs& a, hipStream_t s);
 
 }  // namespace zl

@@ -53,8 +53,10 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
     const int sq = __builtin_amdgcn_readfirstlane(find_tile<16, true>(a, id / a.nsplit, tile));
     if (sq < 0) return;
     const Seq q = seq_of(a, sq);
-    const int r0 = __builtin_amdgcn_readfirstlane(tile) * 16, rows = q.nq * a.gq, r1 = min(r0 + 16, rows) - 1;
-    if (r0 >= rows) return;
+    const int rows = q.nq * a.gq;
+    // the last tiles, whose ranges are the longest, first
+    const int r0 = ((rows + 15) / 16 - 1 - __builtin_amdgcn_readfirstlane(tile)) * 16, r1 = min(r0 + 16, rows) - 1;
+    if (r0 < 0 || r0 >= rows) return;
     const Range rg = tile_range(a, q, r0, r1, a.chunk);
     if (split >= rg.used) return;
     const int ks = rg.ks + split * a.chunk, ke = rg.ke - ks > a.chunk ? ks + a.chunk : rg.ke;
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
 #pragma unroll
             for (int e = 0; e < 4 * NT; ++e) {
                 x[e] = s[e / 4][e % 4];
-                if (a.softcap > 0.0f) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e] * a.scale, a.softcap, a.inv_cap));
+                if (a.softcap > 0.0f) x[e] = cap_bf16(a, x[e]);
             }
         } else {
             // 16 products at a time into a fresh accumulator, these summed in two chains: one chain over the
@@ -331,22 +333,26 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
     }
 }
 
-// Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s, a workgroup
-// each, wave w the splits w, w + 4, ... The row's splits are those of the tile that formed them. The
-// maxima and the first sums are requested before their number is known (slots behind it hold
-// anything: they are dropped, not weighted by 0), which leaves one round trip to memory behind the
-// sequence's own.
+// Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s. W waves take
+// a head, wave w splits w, w + W, ...: four where there can be many splits, one where there are few
+// (and a workgroup four heads). The row's splits are those of the tile that formed them. The maxima
+// and the first sums are requested before their number is known (slots behind it hold anything:
+// they are dropped, not weighted by 0), which leaves one round trip to memory behind the sequence's own.
 constexpr int kMaxSplits = 256;
 constexpr int kJoinWaves = 4;
-template <typename T, int D>
+constexpr int kJoinFew = 16;
+template <typename T, int D, int W>
 __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     constexpr int E = D / 64;  // columns of a lane
-    constexpr int PER = kMaxSplits / kWave;
+    constexpr int PER = W == 1 ? 1 : kMaxSplits / kWave;
     constexpr int PRE = 4;
     typedef float Cols __attribute__((ext_vector_type(E)));
-    __shared__ float s_part[kJoinWaves][D];
+    __shared__ float s_part[W == 1 ? 1 : W][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t th = blockIdx.x, part = th * a.nparts;
+    const int64_t th = W == 1 ? (int64_t)blockIdx.x * kJoinWaves + wave : (int64_t)blockIdx.x;
+    const int w = W == 1 ? 0 : wave;
+    if (th >= (int64_t)a.n_tokens * a.nh) return;  // (uniform in a wave, and in the workgroup where W > 1)
+    const int64_t part = th * a.nparts;
     const int tok = (int)(th / a.nh), h = (int)(th % a.nh);
     const float* const ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
     const float* const sums = a.ws + part * D + E * lane;
@@ -359,7 +365,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     }
     Cols pre[PRE];
 #pragma unroll
-    for (int k = 0; k < PRE; ++k) pre[k] = *reinterpret_cast<const Cols*>(sums + (int64_t)min(wave + k * kJoinWaves, a.nparts - 1) * D);
+    for (int k = 0; k < PRE; ++k) pre[k] = *reinterpret_cast<const Cols*>(sums + (int64_t)min(w + k * W, a.nparts - 1) * D);
     int sq = tok;
     if (a.cu) {
         // the last sequence that begins at or before the token
@@ -401,51 +407,83 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
         for (int j = 1; j < PER; ++j) c = sp / kWave == j ? mv[j] : c;
         return __shfl(c, sp % kWave);
     };
+    for (int s0 = w; s0 < used; s0 += PRE * W) {
+        if (s0 > w) {
 #pragma unroll
-    for (int k = 0; k < PRE; ++k) {
-        const int sp = wave + k * kJoinWaves;
-        if (sp < used) acc += pre[k] * weight(sp);
+            for (int k = 0; k < PRE; ++k) pre[k] = *reinterpret_cast<const Cols*>(sums + (int64_t)min(s0 + k * W, used - 1) * D);
+        }
+#pragma unroll
+        for (int k = 0; k < PRE; ++k)
+            if (s0 + k * W < used) acc += pre[k] * weight(s0 + k * W);
     }
-#pragma unroll 4
-    for (int sp = wave + PRE * kJoinWaves; sp < used; sp += kJoinWaves)
-        acc += *reinterpret_cast<const Cols*>(sums + (int64_t)sp * D) * weight(sp);
-    *reinterpret_cast<Cols*>(&s_part[wave][E * lane]) = acc;
-    __syncthreads();
-    for (int c = threadIdx.x; c < D; c += kJoinWaves * kWave) {
-        const float t = (s_part[0][c] + s_part[1][c]) + (s_part[2][c] + s_part[3][c]);
-        const float v = L == 0.0f ? 0.0f : t / L;
+    auto put = [&](int c, float v) {
+        v = L == 0.0f ? 0.0f : v / L;
         if constexpr (sizeof(T) == 4) ((T*)a.out)[th * D + c] = v;
         else ((T*)a.out)[th * D + c] = (T)(pack_bf16x2(v, 0.0f) & 0xffffu);
+    };
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            put(E * lane + e, acc[e]);
+        }
+    } else {
+        *reinterpret_cast<Cols*>(&s_part[w][E * lane]) = acc;
+        __syncthreads();
+        for (int c = threadIdx.x; c < D; c += kJoinWaves * kWave) put(c, (s_part[0][c] + s_part[1][c]) + (s_part[2][c] + s_part[3][c]));
     }
 }
 
 // ---- host --------------------------------------------------------------------------------------
 
-// Which kernels a call takes, and the splits of each one's ranges. k_seq_tile takes bf16 calls'
-// sequences of more than 16 query rows; a call whose sequences all have that few (a token each), or
-// surely more (a prompt, one chunk), launches one kernel only.
-// Splits have one size in a call, whatever the sequences' lengths, which evens out the workgroups of a ragged
-// batch. k_seq_rows's: half a megabyte of K and V, less where that leaves under 1024 workgroups;
-// k_seq_tile's: where there are under 512 workgroups, down to 256 keys.
+// Which kernels a call takes, and the splits of each one's ranges.
+// k_seq_rows reads K and V for 16 query rows, k_seq_tile for 64 to 256 that share them. Sequences of few rows
+// (bf16 16, f32 64, whose products take ten times as long) are k_seq_rows's, the others k_seq_tile's; a call
+// whose sequences are surely of one kind launches one kernel (32 queries of one sequence behind 4000
+// keys, 8 / 4 heads x 256 f32: 30 us by k_seq_rows, 46 by k_seq_tile; 512 behind 1500: 133 and 114). f32
+// prompts are k_seq_rows's at every length: its workgroups are a quarter of the work and even out (1024
+// tokens 107 us / 219, 4096 724 / 1067).
 static void choose(SeqArgs& a, int dtype) {
+    const bool f32 = dtype == HIP_BRIDGE_F32;
     a.gq = a.nh / a.nkv;
-    a.tile_rows = tile_rows_of(a.D);
+    // Prompts that leave CUs idle take smaller tiles (64 tokens, 8 / 4 heads x 256 bf16 13.4 -> 10.6 us, 512 of 32
+    // / 16 x 128 26 -> 23.5; over the largest, 8192, the larger ones are ahead by 8%).
+    a.tile_rows = tile_rows_of(dtype, a.D, false);
+    if (!a.table && cdiv((int64_t)a.n_tokens * a.gq, a.tile_rows) * a.nkv < 256) a.tile_rows = tile_rows_of(dtype, a.D, true);
     const bool single = a.table && !a.cu;  // a token each
-    if (dtype != HIP_BRIDGE_BF16 || (int64_t)a.n_tokens * a.gq <= 16 || (single && a.gq <= 16)) a.few_rows = INT32_MAX;
-    else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : 16;
-    const int64_t es = dtype == HIP_BRIDGE_F32 ? 4 : 2;
-    auto splits = [&](int R, int64_t wgs, int64_t least, int64_t most, int& chunk) {
-        const int64_t len = most_keys(a, R), groups = most_tiles(a, R) * a.nkv;
-        int64_t keys = std::min(most, cdiv(cdiv(len * groups, wgs), 64) * 64);
-        keys = std::max({keys, least, cdiv(cdiv(len, kMaxSplits), 64) * 64});
+    const int few = f32 ? 64 : 16;
+    const int64_t rows = (int64_t)a.n_tokens * a.gq;
+    if ((f32 && !a.table) || rows <= std::max<int64_t>(few, (int64_t)a.n_seqs * few / 2) || (single && a.gq <= few)) a.few_rows = INT32_MAX;
+    else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : few;
+
+    // A call's splits have one size, whatever the sequences' lengths, which evens out the workgroups of a ragged
+    // batch: `keys` each, or as many more as keep their number within bounds.
+    auto split = [&](int R, int64_t keys, int& chunk) {
+        const int64_t len = most_keys(a, R);
+        keys = std::max(cdiv(keys, 64), cdiv(cdiv(len, kMaxSplits), 64)) * 64;
         chunk = (int)std::min<int64_t>(keys, INT32_MAX);
         return (int)std::max<int64_t>(cdiv(len, keys), 1);
     };
     a.nsplit = a.tile_split = 1;
     a.chunk = a.tile_chunk = INT32_MAX;
-    if (a.few_rows > 0) a.nsplit = splits(16, 1024, 64, (1 << 18) / (a.D * es), a.chunk);
-    if (a.few_rows < INT32_MAX) {
-        if (most_tiles(a, a.tile_rows) * a.nkv < 256) a.tile_split = splits(a.tile_rows, 512, 256, INT32_MAX, a.tile_chunk);
+    if (a.few_rows > 0) {
+        // Decode: half a megabyte of K and V, less where that leaves under 1024 workgroups (16 requests of up to
+        // 8192 positions in 8 equal splits each 188 us, in splits of 256 keys 122), down to a block for each wave (one
+        // token at 1250, f32: 14.6 us in splits of 64 keys, 19.4 of 128), and no more than 16384 workgroups (whose
+        // partial sums take 17 MB at two heads of 128 to a kv head). Chunks: 1024 workgroups.
+        const int64_t groups = most_tiles(a, 16) * a.nkv, all = most_keys(a, 16) * groups, fill = cdiv(all, 1024);
+        const int64_t least = std::max<int64_t>(f32 ? 64 : 128, cdiv(all, 16384));
+        if (a.n_tokens <= a.n_seqs) a.nsplit = split(16, std::max(least, std::min<int64_t>((1 << 18) / (a.D * (f32 ? 4 : 2)), fill)), a.chunk);
+        else if (groups < 1024) a.nsplit = split(16, std::max<int64_t>(fill, 128), a.chunk);
+    }
+    if (a.few_rows < INT32_MAX && a.table) {
+        // Chunks whose tiles (if the sequences are even) leave CUs idle: a workgroup to a CU, or a few where
+        // sequences differ. More splits cost more in partial sums than they even out (bf16, 256 tokens behind 8000,
+        // 32 / 16 heads x 128: 63 us at 256 workgroups, 82 at 512, 116 at 1024), but f32 products last longer
+        // (469, 362, 386 us; 15 chunks of up to 162 tokens behind up to 8400: 1550 at 512, 1277 at 2048).
+        const int64_t tiles = cdiv(rows, a.tile_rows) * a.nkv;
+        const int64_t wgs = f32 ? (a.n_seqs > 1 ? 2048 : 512) : (a.n_seqs > 1 ? 512 : 256);
+        const int64_t least = !f32 && a.n_seqs > 1 ? 256 : 128;
+        if (tiles < 256) a.tile_split = split(a.tile_rows, std::max(least, cdiv(tiles * most_keys(a, a.tile_rows), wgs)), a.tile_chunk);
     }
     a.nparts = std::max(a.nsplit, a.tile_split);
 }
@@ -473,10 +511,11 @@ static void launch_rows(const SeqArgs& a, hipStream_t s) {
         const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
         k_seq_rows<T, D><<<(unsigned)grid, kRowWaves * kWave, 0, s>>>(a);
     }
-    if (a.few_rows < INT32_MAX) launch_tiles(a, s);
+    if (a.few_rows < INT32_MAX) launch_tiles(sizeof(T) == 4 ? HIP_BRIDGE_F32 : HIP_BRIDGE_BF16, a, s);
     if (a.nparts > 1) {
         const int64_t th = (int64_t)a.n_tokens * a.nh;
-        k_seq_join<T, D><<<(unsigned)th, kJoinWaves * kWave, 0, s>>>(a);
+        if (a.nparts <= kJoinFew) k_seq_join<T, D, 1><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
+        else k_seq_join<T, D, kJoinWaves><<<(unsigned)th, kJoinWaves * kWave, 0, s>>>(a);
     }
     check_launch();
 }
@@ -509,6 +548,7 @@ static void launch_seqs(int dtype, SeqArgs& a, void* ws, size_t ws_bytes, hipStr
     }
     a.ws = (float*)ws;
     a.inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    a.cap_in = a.softcap > 0.0f ? 2.0f * kLog2e * (a.scale / a.softcap) : 0.0f;
     // (never 0: a masked score of -inf times it stays -inf)
     a.unit = dtype == HIP_BRIDGE_F32 || a.softcap > 0.0f ? kLog2e : std::max(kLog2e * std::fabs(a.scale), 1e-30f);
     if (most_tiles(a, 16) * a.nkv * a.nparts > INT32_MAX) {

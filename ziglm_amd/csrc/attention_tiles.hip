@@ -51,26 +51,30 @@ __device__ __forceinline__ float over_row(float v, F f) {
     return f(__builtin_bit_cast(float, (unsigned)p[0]), __builtin_bit_cast(float, (unsigned)p[1]));
 }
 
-template <int D, int M, int NW, int KB, int WPE, bool CAP>
+template <typename T, int D, int M, int NW, int KB, int WPE, bool CAP>
 __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     typedef typename Mfma<M>::Acc Acc;
+    constexpr bool BF = sizeof(T) == 2;
+    static_assert(BF || M == 16, "f32 tiles have 16 rows a wave");
+    constexpr int EL = 16 / sizeof(T);   // elements of a 16-byte chunk
+    constexpr int RB = D * sizeof(T);    // bytes of a row
     constexpr int G = 64 / M;            // lanes of a query row
-    constexpr int KD = 8 * G;            // depth of an MFMA
-    constexpr int NQ = D / KD;           // operands of a query row
+    constexpr int NQ = D / (EL * G);     // chunks of a query row to a lane
     constexpr int NT = KB / M;           // score tiles
     constexpr int SR = M * M / 64;       // registers of one
     constexpr int NU = NT * SR / 4;      // groups of four keys of a lane
     constexpr int US = 256 / M;          // keys between them
-    constexpr int NB = D / M;            // column blocks of the output
+    constexpr int NB = D / M;            // accumulators of the output
     constexpr int TH = NW * kWave;
-    constexpr int CR = D / 8;            // 16-byte chunks of a row
+    constexpr int CR = D / EL;           // chunks of a row
     constexpr int NC = KB * CR / TH;     // of a tile, to a thread
     constexpr int RS = TH / CR;          // rows between a thread's chunks
     constexpr float kSlack = 8.0f;       // log2
-    static_assert(KB * CR % TH == 0 && TH % CR == 0 && RS % 8 == 0, "chunks of a tile");
-    constexpr int TB = KB * D * 2;       // bytes of a tile of K or V
+    static_assert(KB * CR % TH == 0 && TH % CR == 0, "chunks of a tile");
+    constexpr int TB = KB * RB;          // bytes of a tile of K or V
     __shared__ __align__(16) uint8_t s_kv[2][2][TB];  // [buffer][K, V]
-    __shared__ uint32_t s_gap[3][KB / 32];  // keys without a row
+    constexpr int GW = (KB + 31) / 32;
+    __shared__ uint32_t s_gap[3][GW];       // keys without a row
     __shared__ int s_wild;                  // infinite or NaN values were kept out of LDS
     const int tid = threadIdx.x, lane = tid & 63, n = lane % M, h = lane / M;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -104,12 +108,12 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     // and of the workgroup's: tiles outside have keys that some rows do not see
     const int wg_lo = a.window > 0 ? max(0, q.pos0 + r1 / a.gq + 1 - a.window) : 0, wg_hi = q.pos0 + r0 / a.gq;
 
-    bf16x8 qv[NQ];
+    u32x4 qv[NQ];
     {
-        const uint16_t* qrow = (const uint16_t*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + 8 * h;
-        const uint32_t flip = !CAP && a.scale < 0.0f ? 0x80008000u : 0u;  // `unit` has no sign
+        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + EL * h;
+        const uint32_t flip = BF && !CAP && a.scale < 0.0f ? 0x80008000u : 0u;  // `unit` has no sign
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) qv[j] = __builtin_bit_cast(bf16x8, ld16(qrow + KD * j) ^ flip);
+        for (int j = 0; j < NQ; ++j) qv[j] = ld16(qrow + EL * G * j) ^ flip;
     }
     Acc o[NB];
 #pragma unroll
@@ -118,17 +122,31 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
 
     // ---- the tiles' way to LDS ----
     const int sr = tid / CR, sc = tid % CR;  // the thread's first row and its chunk of a row
-    const uint16_t* const kbase = (const uint16_t*)a.kc + kvh * D + 8 * sc;
-    const uint16_t* const vbase = (const uint16_t*)a.vc + kvh * D + 8 * sc;
+    const T* const kbase = (const T*)a.kc + kvh * D + EL * sc;
+    const T* const vbase = (const T*)a.vc + kvh * D + EL * sc;
     u32x4 bk[NC], bv[NC];
-    int row[NC];
-    // rows of tile `t` (-1: none, past the range or on a page that is not in the cache)
+    int row[NC], pg[NC];  // cache rows of the tile in bk and bv, page ids of the one behind it
+    // The page ids of tile t are requested behind the loads of the tile before and looked at a tile later (a
+    // wait for them is one for all loads before them).
+    auto find_pages = [&](int t) {
+        if (!a.table) return;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const int key = min(ks + t * KB + sr + j * RS, ke - 1);
+            pg[j] = q.pages[a.page_shift >= 0 ? key >> a.page_shift : key / a.page];
+        }
+    };
+    // rows of tile t from them (-1: none, past the range or on a page that is not in the cache)
     auto find_rows = [&](int t) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int key = ks + t * KB + sr + j * RS;
-            row[j] = row_of(a, q, min(key, ke - 1));
-            if (key >= ke) row[j] = -1;
+            if (a.table) {
+                const int in = a.page_shift >= 0 ? key & (a.page - 1) : key % a.page;
+                row[j] = key < ke && pg[j] >= 0 && pg[j] < a.cache_pages ? pg[j] * a.page + in : -1;
+            } else {
+                row[j] = key < ke ? (int)q.row0 + key : -1;
+            }
         }
     };
     auto load = [&]() {
@@ -139,167 +157,250 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             bv[j] = ld16(vbase + at);
         }
     };
-    // (rows: those of the tile being stored)
-    auto store = [&](int t, const int (&rw)[NC]) {
-        const int buf = t & 1, f = t % 3, k0 = ks + t * KB;
+    auto store = [&](int t) {
+        const int k0 = ks + t * KB;
         bool none = false;
 #pragma unroll
-        for (int j = 0; j < NC; ++j) none |= rw[j] < 0;
+        for (int j = 0; j < NC; ++j) none |= row[j] < 0;
         if (__any(none)) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                if (rw[j] < 0) {
-                    bk[j] = bv[j] = u32x4{};
-                    const int r = sr + j * RS;
-                    if (sc == 0) atomicOr(&s_gap[f][r / 32], 1u << (r % 32));
-                }
+                const int r = sr + j * RS;
+                if (row[j] < 0) bv[j] = u32x4{};
+                if (row[j] < 0 && sc == 0) atomicOr(&s_gap[t % 3][r / 32], 1u << (r % 32));
             }
         }
         if (k0 < wg_lo || k0 + KB - 1 > wg_hi) {
             // Some rows do not see all of the tile's keys: infinite and NaN values, which weights of 0 would
             // carry to them, stay out of LDS, and go to the rows that see them at the end.
+            auto low = [](uint32_t w) { return BF && (w & 0x7f80u) == 0x7f80u; };
+            auto high = [](uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; };
             bool bad = false;
 #pragma unroll
             for (int j = 0; j < NC; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    bad |= (bv[j][e] & 0x7f80u) == 0x7f80u || (bv[j][e] & 0x7f800000u) == 0x7f800000u;
+                for (int e = 0; e < 4; ++e) bad |= low(bv[j][e]) || high(bv[j][e]);
             if (__any(bad)) {
                 if (lane == 0) s_wild = 1;
 #pragma unroll
                 for (int j = 0; j < NC; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if ((bv[j][e] & 0x7f80u) == 0x7f80u) bv[j][e] &= 0xffff0000u;
-                        if ((bv[j][e] & 0x7f800000u) == 0x7f800000u) bv[j][e] &= 0xffffu;
+                        const uint32_t w = bv[j][e];
+                        bv[j][e] = high(w) ? (BF && !low(w) ? w & 0xffffu : 0u) : low(w) ? w & 0xffff0000u : w;
                     }
             }
         }
-        uint8_t* const kd = &s_kv[buf][0][sr * D * 2 + ((sc ^ (sr & 7)) << 4)];
-        uint8_t* const vd = &s_kv[buf][1][sr * D * 2 + ((sc ^ ((sr & 3) << 1)) << 4)];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            *reinterpret_cast<u32x4*>(kd + j * RS * D * 2) = bk[j];
-            *reinterpret_cast<u32x4*>(vd + j * RS * D * 2) = bv[j];
+            const int r = sr + j * RS;
+            *reinterpret_cast<u32x4*>(&s_kv[t & 1][0][r * RB + ((sc ^ (r & 7)) << 4)]) = bk[j];
+            *reinterpret_cast<u32x4*>(&s_kv[t & 1][1][r * RB + ((BF ? sc ^ ((r & 3) << 1) : sc) << 4)]) = bv[j];
         }
     };
+    // Behind tile t: tile t + 1 goes to LDS, the next one's loads out. (Past the last tile row 0 of the cache is
+    // loaded: no load under a branch.)
+    auto stage = [&](int t) {
+        if (t + 1 < ntile) store(t + 1);
+        find_rows(t + 2);
+        load();
+        find_pages(t + 3);
+    };
+
     // The lane's LDS addresses: the swizzle is an exclusive or of the low three bits of a chunk's index,
     // so the operands lie at few bases and offsets that are known here. K: chunk j G + h of row T M + n;
-    // V: chunk b M / 8 + vc (+ 8 bytes) of row u US + 4 h + lane % 16 / 4.
+    // V: chunk b M / 8 + vc (+ 8 bytes) of row u US + 4 h + lane % 16 / 4 (f32: chunk 16 c + n of row
+    // u US + 4 h + r, whole rows by 16 lanes, not swizzled).
     constexpr int KBASES = 8 / G, VBASES = 64 / M;
     const int li = lane & 15;
     const int ky = h ^ (n & 7), vy = ((M == 32 ? 2 * (lane >> 4 & 1) : 0) + ((li & 3) >> 1)) ^ (li >> 2 << 1);
-    const int kn = n * D * 2, vn = (4 * h + (li >> 2)) * D * 2 + (li & 1) * 8;
+    const int kn = n * RB, vn = (4 * h + (li >> 2)) * RB + (li & 1) * 8;
 
-    if (tid == 0) s_wild = 0;
-    if (tid < 3) {
+    float x[NT * SR];          // scores of a tile, then (f32) their weights
+    u32x4 pw[BF ? NU / 2 : 1]; // the weights as operands
+    auto scores = [&](int t) {
+        const uint8_t* kb[KBASES];
 #pragma unroll
-        for (int e = 0; e < KB / 32; ++e) s_gap[tid][e] = 0;
-    }
-    __syncthreads();
-    if (ntile > 0) {
-        int rw[NC];
-        find_rows(0);
-        load();
-#pragma unroll
-        for (int j = 0; j < NC; ++j) rw[j] = row[j];
-        if (ntile > 1) find_rows(1);
-        store(0, rw);
-    }
-    __syncthreads();
-
-    for (int t = 0; t < ntile; ++t) {
-        const int buf = t & 1, f = t % 3, k0 = ks + t * KB;
-        int rw[NC];
-        if (t + 1 < ntile) {  // the next tile's loads, and the rows of the one behind it
-            load();
-#pragma unroll
-            for (int j = 0; j < NC; ++j) rw[j] = row[j];
-            if (t + 2 < ntile) find_rows(t + 2);
-        }
-        if (tid == 0) {  // the flags that tile t - 1 had are tile t + 2's
-#pragma unroll
-            for (int e = 0; e < KB / 32; ++e) s_gap[(t + 2) % 3][e] = 0;
-        }
-        if (k0 <= any_hi && k0 + KB > any_lo) {  // (uniform: some row of the wave sees some key)
-            // scores
-            const uint8_t* kb[KBASES];
-#pragma unroll
-            for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[buf][0][kn + ((c * G ^ ky) << 4)];
+        for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[t & 1][0][kn + ((c * G ^ ky) << 4)];
+        if constexpr (BF) {
             Acc s[NT];
 #pragma unroll
-            for (int T = 0; T < NT; ++T) s[T] = Acc{};
+            for (int z = 0; z < NT; ++z) s[z] = Acc{};
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int T = 0; T < NT; ++T) {
-                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb[j % KBASES] + T * M * D * 2 + (j / KBASES << 7));
-                    s[T] = Mfma<M>::run(kv, qv[j], s[T]);
+                for (int z = 0; z < NT; ++z) {
+                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb[j % KBASES] + z * M * RB + (j / KBASES << 7));
+                    s[z] = Mfma<M>::run(kv, __builtin_bit_cast(bf16x8, qv[j]), s[z]);
                 }
-            float x[NT * SR];
+            // (the reads run ahead of the products)
+            constexpr int AHEAD = NQ * NT < 6 ? NQ * NT : 6;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+            for (int z = 0; z < NQ * NT - AHEAD; ++z) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+#pragma unroll
+            for (int e = 0; e < NT * SR; ++e) x[e] = s[e / SR][e % SR];
+        } else {
+            // 16 products at a time into a fresh accumulator, these summed in two chains (one chain is two to
+            // three times as far from the exact dot product)
+            acc4 s[NT][2];
+#pragma unroll
+            for (int z = 0; z < NT; ++z) s[z][0] = s[z][1] = acc4{};
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int z = 0; z < NT; ++z) {
+                    const f32x4 kv = *reinterpret_cast<const f32x4*>(kb[j % KBASES] + z * M * RB + (j / KBASES << 7));
+                    const f32x4 qf = __builtin_bit_cast(f32x4, qv[j]);
+                    acc4 c = acc4{};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qf[e], c, 0, 0, 0);
+                    s[z][j & 1] += c;
+                }
+#pragma unroll
+            for (int e = 0; e < NT * SR; ++e) x[e] = (s[e / SR][0][e % SR] + s[e / SR][1][e % SR]) * a.scale;
+        }
+    };
+    auto weights = [&](int t) {
+        const int k0 = ks + t * KB;
+        if constexpr (CAP) {
+#pragma unroll
+            for (int e = 0; e < NT * SR; ++e)
+                x[e] = BF ? cap_bf16(a, x[e]) : a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+        }
+        uint32_t gap[GW], some = 0;
+#pragma unroll
+        for (int e = 0; e < GW; ++e) some |= gap[e] = s_gap[t % 3][e];
+        some = __builtin_amdgcn_readfirstlane(some);
+        if (some || !(whole && k0 >= all_lo && k0 + KB - 1 <= all_hi)) {  // uniform
 #pragma unroll
             for (int e = 0; e < NT * SR; ++e) {
-                x[e] = s[e / SR][e % SR];
-                if constexpr (CAP) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e] * a.scale, a.softcap, a.inv_cap));
+                const int kk = e / 4 * US + 4 * h + e % 4, key = k0 + kk;
+                const bool there = !(gap[e / 4 * US / 32] >> (kk % 32) & 1);
+                x[e] = key >= lo && key <= hi && there ? x[e] : -INFINITY;
             }
-            uint32_t gap[KB / 32], some = 0;
+        }
+        float mx = x[0];
 #pragma unroll
-            for (int e = 0; e < KB / 32; ++e) some |= gap[e] = s_gap[f][e];
-            some = __builtin_amdgcn_readfirstlane(some);
-            if (some || !(whole && k0 >= all_lo && k0 + KB - 1 <= all_hi)) {  // uniform
+        for (int e = 1; e < NT * SR; ++e) mx = fmaxf(mx, x[e]);
+        mx = over_row<M>(mx, [](float u, float v) { return fmaxf(u, v); });
+        if (__any(!((mx - m) * a.unit <= kSlack))) {
+            const float mn = fmaxf(m, mx);
+            const float c = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * a.unit);
+            m = mn;
+            l *= c;
 #pragma unroll
-                for (int e = 0; e < NT * SR; ++e) {
-                    const int kk = e / 4 * US + 4 * h + e % 4, key = k0 + kk;
-                    const bool there = !(gap[e / 4 * US / 32] >> (kk % 32) & 1);
-                    x[e] = key >= lo && key <= hi && there ? x[e] : -INFINITY;
-                }
-            }
-            float mx = x[0];
+            for (int b = 0; b < NB; ++b) o[b] *= c;
+        }
+        const float ms = m == -INFINITY ? 0.0f : m, mu = ms * a.unit;
+        float ps = 0.0f;
 #pragma unroll
-            for (int e = 1; e < NT * SR; ++e) mx = fmaxf(mx, x[e]);
-            mx = over_row<M>(mx, [](float u, float v) { return fmaxf(u, v); });
-            if (__any(!((mx - m) * a.unit <= kSlack))) {
-                const float mn = fmaxf(m, mx);
-                const float c = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * a.unit);
-                m = mn;
-                l *= c;
+        for (int e = 0; e < NT * SR; ++e) {
+            // (f32: the difference first, which is nearly exact where it counts)
+            x[e] = __builtin_amdgcn_exp2f(BF ? fmaf(x[e], a.unit, -mu) : (x[e] - ms) * a.unit);
+            ps += x[e];
+        }
+        l += ps;
+        if constexpr (BF) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) o[b] *= c;
-            }
-            const float mu = (m == -INFINITY ? 0.0f : m) * a.unit;
-            float ps = 0.0f;
+            for (int u = 0; u < NU / 2; ++u)
 #pragma unroll
-            for (int e = 0; e < NT * SR; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.unit, -mu));
-                ps += x[e];
-            }
-            l += ps;
-            // output: MFMA t takes key groups 2 t and 2 t + 1
+                for (int e = 0; e < 4; ++e) pw[u][e] = pack_bf16x2(x[8 * u + 2 * e], x[8 * u + 2 * e + 1]);
+        }
+    };
+    auto output = [&](int t) {
+        if constexpr (BF) {
+            // an MFMA takes key groups u and u + 1
             const uint8_t* vb[VBASES];
 #pragma unroll
-            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[buf][1][vn + ((c * (M / 8) ^ vy) << 4)];
+            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[t & 1][1][vn + ((c * (M / 8) ^ vy) << 4)];
 #pragma unroll
             for (int u = 0; u < NU; u += 2) {
-                u32x4 pw;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pw[e] = pack_bf16x2(x[4 * u + 2 * e], x[4 * u + 2 * e + 1]);
-                const bf16x8 pv = __builtin_bit_cast(bf16x8, pw);
+                const bf16x8 pv = __builtin_bit_cast(bf16x8, pw[u / 2]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const uint8_t* const at = vb[b % VBASES] + (b / VBASES << 7);
-                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + u * US * D * 2));
-                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (u + 1) * US * D * 2));
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + u * US * RB));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (u + 1) * US * RB));
                     const bf16x8 vv = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
                     o[b] = Mfma<M>::run(vv, pv, o[b]);
                 }
             }
+            constexpr int ALL = NU / 2 * NB, AHEAD = ALL < 4 ? ALL : 4;
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 1);
+#pragma unroll
+            for (int z = 0; z < ALL - AHEAD; ++z) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 1);
+        } else {
+            // accumulator 4 c + j takes column 64 c + 4 n + j of V, an MFMA keys u US + 4 h + r
+            const uint8_t* const vb = &s_kv[t & 1][1][4 * h * RB + n * 16];
+#pragma unroll
+            for (int e = 0; e < NT * SR; ++e)
+#pragma unroll
+                for (int c = 0; c < NB / 4; ++c) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(vb + (e / 4 * US + e % 4) * RB + c * 256);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], x[e], o[4 * c + j], 0, 0, 0);
+                }
         }
-        if (t + 1 < ntile) store(t + 1, rw);
+    };
+    if (tid == 0) s_wild = 0;
+    if (tid < 3) {
+#pragma unroll
+        for (int e = 0; e < GW; ++e) s_gap[tid][e] = 0;
+    }
+    __syncthreads();
+    if (ntile > 0) {  // (uniform)
+        find_pages(0);
+        find_rows(0);
+        load();
+        find_pages(1);
+        store(0);
+        find_rows(1);
+        load();
+        find_pages(2);
         __syncthreads();
+        for (int t = 0; t < ntile; ++t) {
+            if (tid == 0) {  // the flags that tile t - 1 had are tile t + 2's
+#pragma unroll
+                for (int e = 0; e < GW; ++e) s_gap[(t + 2) % 3][e] = 0;
+            }
+            if (ks + t * KB <= any_hi && ks + t * KB + KB > any_lo) {  // (uniform: some row of the wave sees some key)
+                scores(t);
+                weights(t);
+                output(t);
+            }
+            stage(t);
+            __syncthreads();
+        }
     }
 
     l = over_row<M>(l, [](float u, float v) { return u + v; });
     if (w0 + n > r1) return;
+    // f(column, the lane's four outputs from it on) -> the four
+    auto each4 = [&](auto f) {
+#pragma unroll
+        for (int b = 0; b < NB; b += BF ? 1 : 4)
+#pragma unroll
+            for (int e = 0; e < SR; e += BF ? 4 : 1) {
+                if constexpr (BF) {
+                    const f32x4 v = f(b * M + 2 * e + 4 * h, f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]});
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) o[b][e + z] = v[z];
+                } else {
+                    const f32x4 v = f(16 * b + 16 * h + 4 * e, f32x4{o[b][e], o[b + 1][e], o[b + 2][e], o[b + 3][e]});
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) o[b + z][e] = v[z];
+                }
+            }
+    };
     if (s_wild) {
         // What a row sees of the values kept out: whatever its weight, the value itself.
 #pragma unroll 1
@@ -308,15 +409,13 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             if (k0 >= wg_lo && k0 + KB - 1 <= wg_hi) continue;  // (uniform: the tile went whole)
             const int r = row_of(a, q, k);
             if (r < 0 || k < lo || k > hi) continue;
-            const uint16_t* const vp = (const uint16_t*)a.vc + (int64_t)r * a.kv_stride + kvh * D + 4 * h;
+            const T* const vp = (const T*)a.vc + (int64_t)r * a.kv_stride + kvh * D;
+            each4([&](int col, f32x4 v) {
+                const f32x4 w = ld4(vp + col);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int e = 0; e < SR; e += 4) {
-                    const f32x4 v = ld4(vp + b * M + 2 * e);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) o[b][e + c] += fabsf(v[c]) < INFINITY ? 0.0f : v[c];
-                }
+                for (int z = 0; z < 4; ++z) v[z] += fabsf(w[z]) < INFINITY ? 0.0f : w[z];
+                return v;
+            });
         }
     }
     if (l == 0.0f) {  // no key: zeros, whatever weights of 0 made of the values
@@ -326,20 +425,21 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     }
     const int64_t th = (int64_t)(q.tok0 + i) * a.nh + kvh * a.gq + rr % a.gq;
     if (rg.used == 1) {
+        T* const out = (T*)a.out + th * D;
         const float inv = 1.0f / l;
-        uint16_t* out = (uint16_t*)a.out + th * D + 4 * h;
+        each4([&](int col, f32x4 v) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < SR; e += 4)
-                st4(out + b * M + 2 * e, f32x4{o[b][e] * inv, o[b][e + 1] * inv, o[b][e + 2] * inv, o[b][e + 3] * inv});
+            for (int z = 0; z < 4; ++z) v[z] = BF ? v[z] * inv : v[z] / l;
+            st4(out + col, v);
+            return v;
+        });
     } else {
         const int64_t part = th * a.nparts + split;
-        float* w = a.ws + part * D + 4 * h;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < SR; e += 4) st4(w + b * M + 2 * e, f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]});
+        float* const w = a.ws + part * D;
+        each4([&](int col, f32x4 v) {
+            st4(w + col, v);
+            return v;
+        });
         if (h == 0) {
             float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
             ml[0] = m;
@@ -348,28 +448,35 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     }
 }
 
-template <int D, int M, int NW, int KB, int WPE>
+template <typename T, int D, int M, int NW, int KB, int WPE>
 static void launch(const SeqArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)(most_tiles(a, NW * M) * a.nkv * a.tile_split);
-    if (a.softcap > 0.0f) k_seq_tile<D, M, NW, KB, WPE, true><<<grid, NW * kWave, 0, s>>>(a);
-    else k_seq_tile<D, M, NW, KB, WPE, false><<<grid, NW * kWave, 0, s>>>(a);
+    if (a.softcap > 0.0f) k_seq_tile<T, D, M, NW, KB, WPE, true><<<grid, NW * kWave, 0, s>>>(a);
+    else k_seq_tile<T, D, M, NW, KB, WPE, false><<<grid, NW * kWave, 0, s>>>(a);
 }
 
-#ifndef ZL_T256
-#define ZL_T256 256, 16, 8, 32, 2
-#define ZL_R256 128
-#endif
-#ifndef ZL_T128
-#define ZL_T128 128, 32, 8, 64, 2
-#define ZL_R128 256
-#endif
-int tile_rows_of(int D) { return D <= 64 ? 256 : D == 128 ? ZL_R128 : D == 256 ? ZL_R256 : 128; }
+int tile_rows_of(int dtype, int D, bool small) {
+    if (dtype == HIP_BRIDGE_F32) return 64;
+    return D <= 128 ? (small ? 128 : 256) : D == 256 && small ? 64 : 128;
+}
 
-void launch_tiles(const SeqArgs& a, hipStream_t s) {
-    if (a.D == 64) launch<64, 32, 8, 64, 2>(a, s);
-    else if (a.D == 128) launch<ZL_T128>(a, s);
-    else if (a.D == 256) launch<ZL_T256>(a, s);
-    else launch<512, 16, 8, 32, 2>(a, s);
+void launch_tiles(int dtype, const SeqArgs& a, hipStream_t s) {
+    const bool small = a.tile_rows < tile_rows_of(dtype, a.D, false);
+    if (dtype == HIP_BRIDGE_F32) {
+        if (a.D == 64) launch<float, 64, 16, 4, 32, 2>(a, s);
+        else if (a.D == 128) launch<float, 128, 16, 4, 32, 2>(a, s);
+        else if (a.D == 256) launch<float, 256, 16, 4, 16, 2>(a, s);
+        else launch<float, 512, 16, 4, 16, 1>(a, s);
+    } else if (small) {
+        if (a.D == 64) launch<uint16_t, 64, 32, 4, 64, 2>(a, s);
+        else if (a.D == 128) launch<uint16_t, 128, 32, 4, 64, 2>(a, s);
+        else launch<uint16_t, 256, 16, 4, 32, 2>(a, s);
+    } else {
+        if (a.D == 64) launch<uint16_t, 64, 32, 8, 64, 2>(a, s);
+        else if (a.D == 128) launch<uint16_t, 128, 32, 8, 64, 2>(a, s);
+        else if (a.D == 256) launch<uint16_t, 256, 16, 8, 32, 2>(a, s);
+        else launch<uint16_t, 512, 16, 8, 32, 2>(a, s);
+    }
 }
 
 }  // namespace zl
