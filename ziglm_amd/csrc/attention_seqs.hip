@@ -28,23 +28,30 @@ namespace zl {
 // on its way through the other's product, and two workgroups share a CU, so that one's prologue and
 // merge pass under the other's reads. The waves' states merge through LDS.
 constexpr int kRowWaves = 4;
+// Heads of 512 take two waves to a block of keys, half the head size each, which exchange their sums of the
+// scores through LDS (a wave that had all of it would need all of a SIMD's registers).
+template <int D> constexpr int row_halves() { return D > 256 ? 2 : 1; }
 template <typename T, int D>
-__global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows(SeqArgs a) {
+__global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_rows(SeqArgs a) {
+    constexpr int HV = row_halves<D>(), DW = D / HV;  // of a wave
     constexpr bool BF = sizeof(T) == 2;
     constexpr int BK = BF ? 32 : 16;             // keys of a block
     constexpr int NT = BK / 16;                  // score tiles of it
     constexpr int EL = 16 / sizeof(T);           // elements of a load
-    constexpr int NI = D / (4 * EL);             // K loads of a lane to a tile
+    constexpr int NI = DW / (4 * EL);            // K loads of a lane to a tile
     constexpr int CW = BF && D > 64 ? 8 : 4;     // columns of a V load
-    constexpr int NC = D / (16 * CW);            // V loads of a lane to a row
+    constexpr int NC = DW / (16 * CW);           // V loads of a lane to a row
     constexpr int NR = BF ? 8 : 4;               // V rows of a lane
     constexpr int OS = D + 4;                    // row of the merge buffer
     constexpr int SLOTS = D > 256 ? 2 : 4;
     constexpr float kSlack = 8.0f;               // log2: how far scores may pass the running maximum
-    __shared__ __align__(16) float s_o[SLOTS * 16 * OS];  // (the query rows before)
+    // the merge buffer; before it the query rows, and the halves' sums of the scores
+    __shared__ __align__(16) float s_o[SLOTS * 16 * OS];
+    constexpr int XF = HV * NI * kWave * 4;  // floats of the query rows
+    static_assert(HV == 1 || XF + 2 * HV * kRowWaves * 4 * NT * kWave <= SLOTS * 16 * OS, "LDS");
     __shared__ float s_m[kRowWaves][16], s_l[kRowWaves][16];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wave = wid % kRowWaves, half = wid / kRowWaves;
     int id = (int)blockIdx.x;
     const int kvh = id % a.nkv;
     id /= a.nkv;
@@ -70,9 +77,9 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
     const bool whole = pf >= 0 && pl < q.lim;
     const int all_lo = a.window > 0 ? max(0, pl + 1 - a.window) : 0, all_hi = pf;
 
-    u32x4* const s_q = reinterpret_cast<u32x4*>(s_o) + lane;
+    u32x4* const s_q = reinterpret_cast<u32x4*>(s_o) + half * NI * kWave + lane;
     {
-        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + EL * g;
+        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + half * DW + EL * g;
         const uint32_t flip = BF && !(a.softcap > 0.0f) && a.scale < 0.0f ? 0x80008000u : 0u;  // `unit` has no sign
         for (int j = wave; j < NI; j += kRowWaves) s_q[kWave * j] = ld16(qrow + 4 * EL * j) ^ flip;
     }
@@ -88,8 +95,8 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
         const int key = ks + BK * blk + lane % BK, r = row_of(a, q, min(key, ke - 1));
         return key < ke ? r : -1;
     };
-    const T* const kbase = (const T*)a.kc + kvh * D + EL * g;
-    const T* const vbase = (const T*)a.vc + kvh * D + CW * n;
+    const T* const kbase = (const T*)a.kc + kvh * D + half * DW + EL * g;
+    const T* const vbase = (const T*)a.vc + kvh * D + half * DW + CW * n;
     u32x4 kk[NT][NI];
     typedef uint32_t vload __attribute__((ext_vector_type(BF ? CW / 2 : 4)));
     vload vv[NR][NC];
@@ -114,7 +121,9 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
     load_k(row);
     load_v(row);
     __syncthreads();  // the query rows
-    for (int blk = wave; blk < nblk; blk += kRowWaves) {
+    // (where waves exchange sums all of them go as many steps)
+    const int steps = HV == 1 ? nblk : (nblk + kRowWaves - 1) / kRowWaves * kRowWaves;
+    for (int blk = wave; blk < steps; blk += kRowWaves) {
         const int k0 = ks + BK * blk;
         float x[4 * NT];
         if constexpr (BF) {
@@ -129,10 +138,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
                     s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk[t][j]), qv, s[t], 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4 * NT; ++e) {
-                x[e] = s[e / 4][e % 4];
-                if (a.softcap > 0.0f) x[e] = cap_bf16(a, x[e]);
-            }
+            for (int e = 0; e < 4 * NT; ++e) x[e] = s[e / 4][e % 4];
         } else {
             // 16 products at a time into a fresh accumulator, these summed in two chains: one chain over the
             // whole row is two to three times as far from the exact dot product
@@ -146,10 +152,26 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
                 st[j & 1] += c;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = (st[0][e] + st[1][e]) * a.scale;
-                if (a.softcap > 0.0f) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+            for (int e = 0; e < 4; ++e) x[e] = st[0][e] + st[1][e];
+        }
+        if constexpr (HV > 1) {
+            // (two buffers in turn: a wave is at most a step ahead of its other half)
+            f32x4* const mine = reinterpret_cast<f32x4*>(s_o + XF) + ((blk / kRowWaves & 1) * HV * kRowWaves + wid) * NT * kWave + lane;
+            const f32x4* const other = mine + (half ? -1 : 1) * kRowWaves * NT * kWave;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mine[t * kWave] = f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 y = other[t * kWave];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * t + e] += y[e];
             }
+        }
+#pragma unroll
+        for (int e = 0; e < 4 * NT; ++e) {
+            if constexpr (!BF) x[e] *= a.scale;
+            if (a.softcap > 0.0f) x[e] = BF ? cap_bf16(a, x[e]) : a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
         }
         const int row_v = row;
         __builtin_amdgcn_sched_barrier(0);  // the loads stay behind the last use of their registers
@@ -251,7 +273,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
             if (k / BK % kRowWaves != wave || key >= ke) continue;
             const int r = row_of(a, q, key);
             if (r < 0 || key < lo || key > hi) continue;
-            const T* const vp = (const T*)a.vc + (int64_t)r * a.kv_stride + kvh * D + 4 * CW * g;
+            const T* const vp = (const T*)a.vc + (int64_t)r * a.kv_stride + kvh * D + half * DW + 4 * CW * g;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -273,7 +295,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
 #pragma unroll
         for (int j = 0; j < NC * CW; ++j) o[j] = acc4{};
     }
-    if (g == 0) {
+    if (g == 0 && half == 0) {
         s_m[wave][n] = m;
         s_l[wave][n] = l;
     }
@@ -286,7 +308,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
 #pragma unroll
         for (int j = 0; j < NC * CW; ++j) o[j] *= f;
     }
-    float* const slot = s_o + (wave % SLOTS * 16 + n) * OS + 4 * CW * g;
+    float* const slot = s_o + (wave % SLOTS * 16 + n) * OS + half * DW + 4 * CW * g;
 #pragma unroll
     for (int w0 = 0; w0 < kRowWaves; w0 += SLOTS) {
         if (wave >= w0 && wave < w0 + SLOTS && r0 + n <= r1) {
@@ -304,7 +326,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, D > 256 ? 1 : 2) void k_seq_rows
         }
         __syncthreads();
     }
-    for (int t = threadIdx.x; t < 16 * D / 4; t += kRowWaves * kWave) {
+    for (int t = threadIdx.x; t < 16 * D / 4; t += HV * kRowWaves * kWave) {
         const int rw = t / (D / 4), col = t % (D / 4) * 4;
         if (r0 + rw > r1) break;
         const int64_t tok = q.tok0 + (r0 + rw) / a.gq, h = kvh * a.gq + (r0 + rw) % a.gq;
@@ -509,7 +531,7 @@ template <typename T, int D>
 static void launch_rows(const SeqArgs& a, hipStream_t s) {
     if (a.few_rows > 0) {
         const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
-        k_seq_rows<T, D><<<(unsigned)grid, kRowWaves * kWave, 0, s>>>(a);
+        k_seq_rows<T, D><<<(unsigned)grid, row_halves<D>() * kRowWaves * kWave, 0, s>>>(a);
     }
     if (a.few_rows < INT32_MAX) launch_tiles(sizeof(T) == 4 ? HIP_BRIDGE_F32 : HIP_BRIDGE_BF16, a, s);
     if (a.nparts > 1) {

@@ -51,20 +51,22 @@ __device__ __forceinline__ float over_row(float v, F f) {
     return f(__builtin_bit_cast(float, (unsigned)p[0]), __builtin_bit_cast(float, (unsigned)p[1]));
 }
 
-template <typename T, int D, int M, int NW, int KB, int WPE, bool CAP>
-__global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
+template <typename T, int D, int M, int NW, int KB, int HV, bool CAP>
+__global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     typedef typename Mfma<M>::Acc Acc;
     constexpr bool BF = sizeof(T) == 2;
     static_assert(BF || M == 16, "f32 tiles have 16 rows a wave");
     constexpr int EL = 16 / sizeof(T);   // elements of a 16-byte chunk
     constexpr int RB = D * sizeof(T);    // bytes of a row
     constexpr int G = 64 / M;            // lanes of a query row
-    constexpr int NQ = D / (EL * G);     // chunks of a query row to a lane
+    constexpr int DW = D / HV;           // of the head size, a wave's part
+    constexpr int RG = NW / HV;          // groups of M query rows
+    constexpr int NQ = DW / (EL * G);    // chunks of a query row to a lane
     constexpr int NT = KB / M;           // score tiles
     constexpr int SR = M * M / 64;       // registers of one
     constexpr int NU = NT * SR / 4;      // groups of four keys of a lane
     constexpr int US = 256 / M;          // keys between them
-    constexpr int NB = D / M;            // accumulators of the output
+    constexpr int NB = DW / M;           // accumulators of the output
     constexpr int TH = NW * kWave;
     constexpr int CR = D / EL;           // chunks of a row
     constexpr int NC = KB * CR / TH;     // of a tile, to a thread
@@ -75,29 +77,30 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     __shared__ __align__(16) uint8_t s_kv[2][2][TB];  // [buffer][K, V]
     constexpr int GW = (KB + 31) / 32;
     __shared__ uint32_t s_gap[3][GW];       // keys without a row
+    __shared__ f32x4 s_x[HV > 1 ? NW : 1][NU][kWave];  // the halves' sums of the scores
     __shared__ int s_wild;                  // infinite or NaN values were kept out of LDS
     const int tid = threadIdx.x, lane = tid & 63, n = lane % M, h = lane / M;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave / RG;
     int id = (int)blockIdx.x;
     const int kvh = id % a.nkv;
     id /= a.nkv;
     const int split = id % a.tile_split;
     int tile;
-    const int sq = __builtin_amdgcn_readfirstlane(find_tile<NW * M, false>(a, id / a.tile_split, tile));
+    const int sq = __builtin_amdgcn_readfirstlane(find_tile<RG * M, false>(a, id / a.tile_split, tile));
     if (sq < 0) return;
     const Seq q = seq_of(a, sq);
     const int rows = q.nq * a.gq;
     // the last tiles, whose ranges are the longest, first
-    const int r0 = ((rows + NW * M - 1) / (NW * M) - 1 - __builtin_amdgcn_readfirstlane(tile)) * (NW * M);
+    const int r0 = ((rows + RG * M - 1) / (RG * M) - 1 - __builtin_amdgcn_readfirstlane(tile)) * (RG * M);
     if (r0 < 0 || r0 >= rows) return;
-    const int r1 = min(r0 + NW * M, rows) - 1;
+    const int r1 = min(r0 + RG * M, rows) - 1;
     const Range rg = tile_range(a, q, r0, r1, a.tile_chunk);
     if (split >= rg.used) return;
     const int ks = rg.ks + split * a.tile_chunk, ke = rg.ke - ks > a.tile_chunk ? ks + a.tile_chunk : rg.ke;
     const int ntile = ke > ks ? (ke - ks + KB - 1) / KB : 0;
 
     // the lane's query row and its keys [lo, hi], and what all of the wave's rows see
-    const int w0 = r0 + wave * M, w1 = min(w0 + M - 1, r1);
+    const int w0 = r0 + wave % RG * M, w1 = min(w0 + M - 1, r1);
     const int rr = min(w0 + n, r1), i = rr / a.gq, p = q.pos0 + i;
     const int hi = p >= 0 && p < q.lim ? p : -1;  // (rows behind the last are the last once more)
     const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
 
     u32x4 qv[NQ];
     {
-        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + EL * h;
+        const T* qrow = (const T*)a.q + (int64_t)(q.tok0 + i) * a.q_stride + (kvh * a.gq + rr % a.gq) * D + half * DW + EL * h;
         const uint32_t flip = BF && !CAP && a.scale < 0.0f ? 0x80008000u : 0u;  // `unit` has no sign
 #pragma unroll
         for (int j = 0; j < NQ; ++j) qv[j] = ld16(qrow + EL * G * j) ^ flip;
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     auto scores = [&](int t) {
         const uint8_t* kb[KBASES];
 #pragma unroll
-        for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[t & 1][0][kn + ((c * G ^ ky) << 4)];
+        for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[t & 1][0][half * DW * (int)sizeof(T) + kn + ((c * G ^ ky) << 4)];
         if constexpr (BF) {
             Acc s[NT];
 #pragma unroll
@@ -262,15 +265,23 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
                     s[z][j & 1] += c;
                 }
 #pragma unroll
-            for (int e = 0; e < NT * SR; ++e) x[e] = (s[e / SR][0][e % SR] + s[e / SR][1][e % SR]) * a.scale;
+            for (int e = 0; e < NT * SR; ++e) x[e] = s[e / SR][0][e % SR] + s[e / SR][1][e % SR];
         }
     };
     auto weights = [&](int t) {
         const int k0 = ks + t * KB;
-        if constexpr (CAP) {
+        if constexpr (HV > 1) {
 #pragma unroll
-            for (int e = 0; e < NT * SR; ++e)
-                x[e] = BF ? cap_bf16(a, x[e]) : a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+            for (int u = 0; u < NU; ++u) {
+                const f32x4 y = s_x[(wave + RG) % NW][u][lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * u + e] += y[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NT * SR; ++e) {
+            if constexpr (!BF) x[e] *= a.scale;
+            if constexpr (CAP) x[e] = BF ? cap_bf16(a, x[e]) : a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
         }
         uint32_t gap[GW], some = 0;
 #pragma unroll
@@ -317,7 +328,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             // an MFMA takes key groups u and u + 1
             const uint8_t* vb[VBASES];
 #pragma unroll
-            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[t & 1][1][vn + ((c * (M / 8) ^ vy) << 4)];
+            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[t & 1][1][half * DW * (int)sizeof(T) + vn + ((c * (M / 8) ^ vy) << 4)];
 #pragma unroll
             for (int u = 0; u < NU; u += 2) {
                 const bf16x8 pv = __builtin_bit_cast(bf16x8, pw[u / 2]);
@@ -340,7 +351,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 1);
         } else {
             // accumulator 4 c + j takes column 64 c + 4 n + j of V, an MFMA keys u US + 4 h + r
-            const uint8_t* const vb = &s_kv[t & 1][1][4 * h * RB + n * 16];
+            const uint8_t* const vb = &s_kv[t & 1][1][half * DW * (int)sizeof(T) + 4 * h * RB + n * 16];
 #pragma unroll
             for (int e = 0; e < NT * SR; ++e)
 #pragma unroll
@@ -372,8 +383,16 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
 #pragma unroll
                 for (int e = 0; e < GW; ++e) s_gap[(t + 2) % 3][e] = 0;
             }
-            if (ks + t * KB <= any_hi && ks + t * KB + KB > any_lo) {  // (uniform: some row of the wave sees some key)
-                scores(t);
+            const bool some = ks + t * KB <= any_hi && ks + t * KB + KB > any_lo;  // (uniform: some row of the wave sees some key)
+            if (some) scores(t);
+            if constexpr (HV > 1) {
+                if (some) {
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) s_x[wave][u][lane] = f32x4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
+                }
+                __syncthreads();
+            }
+            if (some) {
                 weights(t);
                 output(t);
             }
@@ -391,11 +410,11 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
 #pragma unroll
             for (int e = 0; e < SR; e += BF ? 4 : 1) {
                 if constexpr (BF) {
-                    const f32x4 v = f(b * M + 2 * e + 4 * h, f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]});
+                    const f32x4 v = f(half * DW + b * M + 2 * e + 4 * h, f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]});
 #pragma unroll
                     for (int z = 0; z < 4; ++z) o[b][e + z] = v[z];
                 } else {
-                    const f32x4 v = f(16 * b + 16 * h + 4 * e, f32x4{o[b][e], o[b + 1][e], o[b + 2][e], o[b + 3][e]});
+                    const f32x4 v = f(half * DW + 16 * b + 16 * h + 4 * e, f32x4{o[b][e], o[b + 1][e], o[b + 2][e], o[b + 3][e]});
 #pragma unroll
                     for (int z = 0; z < 4; ++z) o[b + z][e] = v[z];
                 }
@@ -440,7 +459,7 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
             st4(w + col, v);
             return v;
         });
-        if (h == 0) {
+        if (h == 0 && half == 0) {
             float* ml = a.ws + (int64_t)a.n_tokens * a.nh * a.nparts * D + 2 * part;
             ml[0] = m;
             ml[1] = l;
@@ -448,34 +467,35 @@ __global__ __launch_bounds__(NW * kWave, WPE) void k_seq_tile(SeqArgs a) {
     }
 }
 
-template <typename T, int D, int M, int NW, int KB, int WPE>
+template <typename T, int D, int M, int NW, int KB, int HV = 1>
 static void launch(const SeqArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)(most_tiles(a, NW * M) * a.nkv * a.tile_split);
-    if (a.softcap > 0.0f) k_seq_tile<T, D, M, NW, KB, WPE, true><<<grid, NW * kWave, 0, s>>>(a);
-    else k_seq_tile<T, D, M, NW, KB, WPE, false><<<grid, NW * kWave, 0, s>>>(a);
+    const unsigned grid = (unsigned)(most_tiles(a, NW / HV * M) * a.nkv * a.tile_split);
+    if (a.softcap > 0.0f) k_seq_tile<T, D, M, NW, KB, HV, true><<<grid, NW * kWave, 0, s>>>(a);
+    else k_seq_tile<T, D, M, NW, KB, HV, false><<<grid, NW * kWave, 0, s>>>(a);
 }
 
 int tile_rows_of(int dtype, int D, bool small) {
-    if (dtype == HIP_BRIDGE_F32) return 64;
-    return D <= 128 ? (small ? 128 : 256) : D == 256 && small ? 64 : 128;
+    if (dtype == HIP_BRIDGE_F32 || D == 512) return 64;
+    return D <= 128 ? (small ? 128 : 256) : small ? 64 : 128;
 }
 
 void launch_tiles(int dtype, const SeqArgs& a, hipStream_t s) {
     const bool small = a.tile_rows < tile_rows_of(dtype, a.D, false);
     if (dtype == HIP_BRIDGE_F32) {
-        if (a.D == 64) launch<float, 64, 16, 4, 32, 2>(a, s);
-        else if (a.D == 128) launch<float, 128, 16, 4, 32, 2>(a, s);
-        else if (a.D == 256) launch<float, 256, 16, 4, 16, 2>(a, s);
-        else launch<float, 512, 16, 4, 16, 1>(a, s);
+        if (a.D == 64) launch<float, 64, 16, 4, 32>(a, s);
+        else if (a.D == 128) launch<float, 128, 16, 4, 32>(a, s);
+        else if (a.D == 256) launch<float, 256, 16, 4, 16>(a, s);
+        else launch<float, 512, 16, 8, 16, 2>(a, s);
+    } else if (a.D == 512) {
+        launch<uint16_t, 512, 16, 8, 32, 2>(a, s);
     } else if (small) {
-        if (a.D == 64) launch<uint16_t, 64, 32, 4, 64, 2>(a, s);
-        else if (a.D == 128) launch<uint16_t, 128, 32, 4, 64, 2>(a, s);
-        else launch<uint16_t, 256, 16, 4, 32, 2>(a, s);
+        if (a.D == 64) launch<uint16_t, 64, 32, 4, 64>(a, s);
+        else if (a.D == 128) launch<uint16_t, 128, 32, 4, 64>(a, s);
+        else launch<uint16_t, 256, 16, 4, 32>(a, s);
     } else {
-        if (a.D == 64) launch<uint16_t, 64, 32, 8, 64, 2>(a, s);
-        else if (a.D == 128) launch<uint16_t, 128, 32, 8, 64, 2>(a, s);
-        else if (a.D == 256) launch<uint16_t, 256, 16, 8, 32, 2>(a, s);
-        else launch<uint16_t, 512, 16, 8, 32, 2>(a, s);
+        if (a.D == 64) launch<uint16_t, 64, 32, 8, 64>(a, s);
+        else if (a.D == 128) launch<uint16_t, 128, 32, 8, 64>(a, s);
+        else launch<uint16_t, 256, 16, 8, 32>(a, s);
     }
 }
 
