@@ -234,10 +234,15 @@ __global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_
             wild |= __any(bad) != 0;
         }
         if constexpr (BF) {
-            u32x4 pw;
+            // the weights as two bf16 terms (16 bits; one alone would add an error as large as the output's own
+            // rounding, and the products here wait for memory anyway)
+            u32x4 ph, pl;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pw[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
-            const bf16x8 pv = __builtin_bit_cast(bf16x8, pw);
+            for (int e = 0; e < 4; ++e) {
+                ph[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+                pl[e] = pack_bf16x2(x[2 * e] - bf16_lo(ph[e]), x[2 * e + 1] - bf16_hi(ph[e]));
+            }
+            const bf16x8 pv = __builtin_bit_cast(bf16x8, ph), pr = __builtin_bit_cast(bf16x8, pl);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -248,9 +253,12 @@ __global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_
                         v0[e] = __builtin_amdgcn_perm(vv[2 * e + 1][c][w], vv[2 * e][c][w], 0x05040100u);
                         v1[e] = __builtin_amdgcn_perm(vv[2 * e + 1][c][w], vv[2 * e][c][w], 0x07060302u);
                     }
+                    const bf16x8 b0 = __builtin_bit_cast(bf16x8, v0), b1 = __builtin_bit_cast(bf16x8, v1);
                     acc4 &o0 = o[c * CW + 2 * w], &o1 = o[c * CW + 2 * w + 1];
-                    o0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v0), pv, o0, 0, 0, 0);
-                    o1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v1), pv, o1, 0, 0, 0);
+                    o0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b0, pr, o0, 0, 0, 0);
+                    o1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b1, pr, o1, 0, 0, 0);
+                    o0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b0, pv, o0, 0, 0, 0);
+                    o1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b1, pv, o1, 0, 0, 0);
                 }
         } else {
 #pragma unroll

@@ -10,8 +10,7 @@
 // tile's scores the lane (n, h = lane / M) holds keys u * 256 / M + 4 h + {0..3}, u = 0, 1, ..: groups
 // of four keys, which is also what a transposing LDS read (ds_read_b64_tr_b16: lane i of 16 gets column i
 // of four rows) gives of V, row-major as it is in the cache. The two products order their keys alike.
-// LDS rows are swizzled by 16-byte chunks, K's by row % 8 (16-byte reads of 8 rows at one column), V's
-// by 2 (row % 4) (4 rows by 32 bytes of a transposing read). K and V of the next tile are on their way
+// K and V of the next tile are on their way
 // to registers while a tile is computed, and go to the other LDS buffer behind it: one barrier a tile.
 // The weights round to bf16 for the second product (half a step, 2^-8 relative, as the output does); their
 // sum takes them unrounded. The running maximum moves only when a row exceeds it by 8 in the exponent
@@ -73,8 +72,11 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     constexpr int RS = TH / CR;          // rows between a thread's chunks
     constexpr float kSlack = 8.0f;       // log2
     static_assert(KB * CR % TH == 0 && TH % CR == 0, "chunks of a tile");
-    constexpr int TB = KB * RB;          // bytes of a tile of K or V
-    __shared__ __align__(16) uint8_t s_kv[2][2][TB];  // [buffer][K, V]
+    // LDS rows are padded so that no two lanes of a phase (16 of a 16-byte read, 32 of an 8-byte one) meet in a
+    // bank: K's by 16 bytes (16 rows at one column), V's for transposing reads of 4 rows and 32 bytes a group
+    // of 16 lanes, whose other group has the next 32 bytes (M 32: 64 bytes) or the next rows (M 16: 32).
+    constexpr int KS = RB + 16, VS = RB + (!BF ? 0 : M == 32 ? 64 : 32);
+    __shared__ __align__(16) uint8_t s_k[2][KB * KS], s_v[2][KB * VS];
     constexpr int GW = (KB + 31) / 32;
     __shared__ uint32_t s_gap[3][GW];       // keys without a row
     __shared__ f32x4 s_x[HV > 1 ? NW : 1][NU][kWave];  // the halves' sums of the scores
@@ -197,8 +199,8 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int r = sr + j * RS;
-            *reinterpret_cast<u32x4*>(&s_kv[t & 1][0][r * RB + ((sc ^ (r & 7)) << 4)]) = bk[j];
-            *reinterpret_cast<u32x4*>(&s_kv[t & 1][1][r * RB + ((BF ? sc ^ ((r & 3) << 1) : sc) << 4)]) = bv[j];
+            *reinterpret_cast<u32x4*>(&s_k[t & 1][r * KS + 16 * sc]) = bk[j];
+            *reinterpret_cast<u32x4*>(&s_v[t & 1][r * VS + 16 * sc]) = bv[j];
         }
     };
     // Behind tile t: tile t + 1 goes to LDS, the next one's loads out. (Past the last tile row 0 of the cache is
@@ -210,21 +212,16 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
         find_pages(t + 3);
     };
 
-    // The lane's LDS addresses: the swizzle is an exclusive or of the low three bits of a chunk's index,
-    // so the operands lie at few bases and offsets that are known here. K: chunk j G + h of row T M + n;
-    // V: chunk b M / 8 + vc (+ 8 bytes) of row u US + 4 h + lane % 16 / 4 (f32: chunk 16 c + n of row
-    // u US + 4 h + r, whole rows by 16 lanes, not swizzled).
-    constexpr int KBASES = 8 / G, VBASES = 64 / M;
-    const int li = lane & 15;
-    const int ky = h ^ (n & 7), vy = ((M == 32 ? 2 * (lane >> 4 & 1) : 0) + ((li & 3) >> 1)) ^ (li >> 2 << 1);
-    const int kn = n * RB, vn = (4 * h + (li >> 2)) * RB + (li & 1) * 8;
+    // The lane's LDS addresses: K, chunk j G + h of row T M + n; V, chunk b M / 8 + .. of row u US + 4 h + li / 4
+    // (f32: chunk 16 c + n of row u US + 4 h + r).
+    const int li = lane & 15, at_half = half * DW * (int)sizeof(T);
+    const int ka = at_half + n * KS + 16 * h;
+    const int va = at_half + (BF ? (4 * h + (li >> 2)) * VS + (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (li & 3) : 4 * h * VS + 16 * n);
 
     float x[NT * SR];          // scores of a tile, then (f32) their weights
     u32x4 pw[BF ? NU / 2 : 1]; // the weights as operands
     auto scores = [&](int t) {
-        const uint8_t* kb[KBASES];
-#pragma unroll
-        for (int c = 0; c < KBASES; ++c) kb[c] = &s_kv[t & 1][0][half * DW * (int)sizeof(T) + kn + ((c * G ^ ky) << 4)];
+        const uint8_t* const kb = &s_k[t & 1][ka];
         if constexpr (BF) {
             Acc s[NT];
 #pragma unroll
@@ -233,7 +230,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int z = 0; z < NT; ++z) {
-                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb[j % KBASES] + z * M * RB + (j / KBASES << 7));
+                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb + z * M * KS + j * G * 16);
                     s[z] = Mfma<M>::run(kv, __builtin_bit_cast(bf16x8, qv[j]), s[z]);
                 }
             // (the reads run ahead of the products)
@@ -257,7 +254,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int z = 0; z < NT; ++z) {
-                    const f32x4 kv = *reinterpret_cast<const f32x4*>(kb[j % KBASES] + z * M * RB + (j / KBASES << 7));
+                    const f32x4 kv = *reinterpret_cast<const f32x4*>(kb + z * M * KS + j * G * 16);
                     const f32x4 qf = __builtin_bit_cast(f32x4, qv[j]);
                     acc4 c = acc4{};
 #pragma unroll
@@ -326,17 +323,15 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     auto output = [&](int t) {
         if constexpr (BF) {
             // an MFMA takes key groups u and u + 1
-            const uint8_t* vb[VBASES];
-#pragma unroll
-            for (int c = 0; c < VBASES; ++c) vb[c] = &s_kv[t & 1][1][half * DW * (int)sizeof(T) + vn + ((c * (M / 8) ^ vy) << 4)];
+            const uint8_t* const vb = &s_v[t & 1][va];
 #pragma unroll
             for (int u = 0; u < NU; u += 2) {
                 const bf16x8 pv = __builtin_bit_cast(bf16x8, pw[u / 2]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const uint8_t* const at = vb[b % VBASES] + (b / VBASES << 7);
-                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + u * US * RB));
-                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (u + 1) * US * RB));
+                    const uint8_t* const at = vb + b * M * 2;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + u * US * VS));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (u + 1) * US * VS));
                     const bf16x8 vv = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
                     o[b] = Mfma<M>::run(vv, pv, o[b]);
                 }
@@ -351,12 +346,12 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 1);
         } else {
             // accumulator 4 c + j takes column 64 c + 4 n + j of V, an MFMA keys u US + 4 h + r
-            const uint8_t* const vb = &s_kv[t & 1][1][half * DW * (int)sizeof(T) + 4 * h * RB + n * 16];
+            const uint8_t* const vb = &s_v[t & 1][va];
 #pragma unroll
             for (int e = 0; e < NT * SR; ++e)
 #pragma unroll
                 for (int c = 0; c < NB / 4; ++c) {
-                    const f32x4 v = *reinterpret_cast<const f32x4*>(vb + (e / 4 * US + e % 4) * RB + c * 256);
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(vb + (e / 4 * US + e % 4) * VS + c * 256);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], x[e], o[4 * c + j], 0, 0, 0);
                 }
