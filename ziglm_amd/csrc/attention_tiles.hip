@@ -72,11 +72,16 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     constexpr int RS = TH / CR;          // rows between a thread's chunks
     constexpr float kSlack = 8.0f;       // log2
     static_assert(KB * CR % TH == 0 && TH % CR == 0, "chunks of a tile");
-    // LDS rows are padded so that no two lanes of a phase (16 of a 16-byte read, 32 of an 8-byte one) meet in a
-    // bank: K's by 16 bytes (16 rows at one column), V's for transposing reads of 4 rows and 32 bytes a group
-    // of 16 lanes, whose other group has the next 32 bytes (M 32: 64 bytes) or the next rows (M 16: 32).
-    constexpr int KS = RB + 16, VS = RB + (!BF ? 0 : M == 32 ? 64 : 32);
-    __shared__ __align__(16) uint8_t s_k[2][KB * KS], s_v[2][KB * VS];
+    // LDS is laid out so that no two lanes of a phase meet in a bank (a phase of a 16-byte read has 16 lanes: 0-3,
+    // 12-15, 20-27 or 4-11, 16-19, 28-31 of a half wave; of an 8-byte read 32). K: M 32 reads 16 rows at one
+    // column in a phase, rows are padded by 16 bytes; M 16 reads 8 rows at one chunk and the others at the
+    // next, so the chunks stand in four planes by their index mod 4, rows padded to an odd number of chunks.
+    // V: a transposing read has 4 rows and 32 bytes a group of 16 lanes, and in the other group the next 32
+    // bytes (M 32: rows padded by 64 bytes) or the next rows (M 16: by 32).
+    constexpr int PLANES = M == 32 ? 1 : 4;
+    constexpr int KS = RB / PLANES + 16, KP = KB * KS, VS = RB + (!BF ? 0 : M == 32 ? 64 : 32);
+    static_assert(M == 32 || (KP % 256 == 0 && KS / 16 % 2 == 1), "planes");
+    __shared__ __align__(16) uint8_t s_k[2][PLANES * KP], s_v[2][KB * VS];
     constexpr int GW = (KB + 31) / 32;
     __shared__ uint32_t s_gap[3][GW];       // keys without a row
     __shared__ f32x4 s_x[HV > 1 ? NW : 1][NU][kWave];  // the halves' sums of the scores
@@ -127,7 +132,9 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
 
     // ---- the tiles' way to LDS ----
     const int sr = tid / CR, sc = tid % CR;  // the thread's first row and its chunk of a row
-    const T* const kbase = (const T*)a.kc + kvh * D + EL * sc;
+    const int kc = sc % (CR / PLANES) * PLANES + sc / (CR / PLANES);  // its chunk of K
+    const int kst = sr * KS + kc % PLANES * KP + kc / PLANES * 16;
+    const T* const kbase = (const T*)a.kc + kvh * D + EL * kc;
     const T* const vbase = (const T*)a.vc + kvh * D + EL * sc;
     u32x4 bk[NC], bv[NC];
     int row[NC], pg[NC];  // cache rows of the tile in bk and bv, page ids of the one behind it
@@ -199,7 +206,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int r = sr + j * RS;
-            *reinterpret_cast<u32x4*>(&s_k[t & 1][r * KS + 16 * sc]) = bk[j];
+            *reinterpret_cast<u32x4*>(&s_k[t & 1][kst + j * RS * KS]) = bk[j];
             *reinterpret_cast<u32x4*>(&s_v[t & 1][r * VS + 16 * sc]) = bv[j];
         }
     };
@@ -212,10 +219,10 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
         find_pages(t + 3);
     };
 
-    // The lane's LDS addresses: K, chunk j G + h of row T M + n; V, chunk b M / 8 + .. of row u US + 4 h + li / 4
+    // The lane's LDS addresses: K, chunk j G + h of row z M + n; V, chunk b M / 8 + .. of row u US + 4 h + li / 4
     // (f32: chunk 16 c + n of row u US + 4 h + r).
     const int li = lane & 15, at_half = half * DW * (int)sizeof(T);
-    const int ka = at_half + n * KS + 16 * h;
+    const int ka = at_half / PLANES + n * KS + (M == 32 ? 16 : KP) * h;
     const int va = at_half + (BF ? (4 * h + (li >> 2)) * VS + (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (li & 3) : 4 * h * VS + 16 * n);
 
     float x[NT * SR];          // scores of a tile, then (f32) their weights
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int z = 0; z < NT; ++z) {
-                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb + z * M * KS + j * G * 16);
+                    const bf16x8 kv = *reinterpret_cast<const bf16x8*>(kb + z * M * KS + j * G * 16 / PLANES);
                     s[z] = Mfma<M>::run(kv, __builtin_bit_cast(bf16x8, qv[j]), s[z]);
                 }
             // (the reads run ahead of the products)
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int z = 0; z < NT; ++z) {
-                    const f32x4 kv = *reinterpret_cast<const f32x4*>(kb + z * M * KS + j * G * 16);
+                    const f32x4 kv = *reinterpret_cast<const f32x4*>(kb + z * M * KS + j * G * 16 / PLANES);
                     const f32x4 qf = __builtin_bit_cast(f32x4, qv[j]);
                     acc4 c = acc4{};
 #pragma unroll
