@@ -26,7 +26,7 @@ LIB = os.path.join(PKG, "libhip_bridge.so")
 ORACLE_DIR = os.path.join(ROOT, "oracle")
 
 SOURCES = ["runtime.hip", "embed.hip", "norm.hip", "rope_kv.hip", "elementwise.hip", "gemv.hip", "gemm.hip",
-           "attention.hip", "attention_seqs.hip", "attention_tiles.hip", "paged_plan.hip", "argmax.hip", "stream.hip", "gguf.cpp"]
+           "attention.hip", "attention_seqs.hip", "attention_tiles.hip", "attention_terms.hip", "paged_plan.hip", "argmax.hip", "stream.hip", "gguf.cpp"]
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 

@@ -153,5 +153,6 @@ inline int64_t most_tiles(const SeqArgs& a, int R) {
 // k_seq_tile (attention_tiles.hip): query rows of a workgroup for a type and head size, and the launch.
 int tile_rows_of(int dtype, int D, bool small);
 void launch_tiles(int dtype, const SeqArgs& a, hipStream_t s);
+void launch_terms(const SeqArgs& a, hipStream_t s);  // (attention_terms.hip)
 
 }  // namespace zl

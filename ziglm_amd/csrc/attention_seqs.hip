@@ -466,23 +466,25 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
 // ---- host --------------------------------------------------------------------------------------
 
 // Which kernels a call takes, and the splits of each one's ranges.
-// k_seq_rows reads K and V for 16 query rows, k_seq_tile for 64 to 256 that share them. Sequences of few rows
-// (bf16 16, f32 64, whose products take ten times as long) are k_seq_rows's, the others k_seq_tile's; a call
-// whose sequences are surely of one kind launches one kernel (32 queries of one sequence behind 4000
-// keys, 8 / 4 heads x 256 f32: 30 us by k_seq_rows, 46 by k_seq_tile; 512 behind 1500: 133 and 114). f32
-// prompts are k_seq_rows's at every length: its workgroups are a quarter of the work and even out (1024
-// tokens 107 us / 219, 4096 724 / 1067).
+// k_seq_rows reads K and V for 16 query rows; the tile kernels (k_seq_tile; f32 heads up to 256 k_seq_terms)
+// for 64 to 256 that share them. Sequences of few rows (bf16 16, f32 64) are k_seq_rows's, the others the
+// tiles'; a call whose sequences are surely of one kind launches one kernel (32 queries of one sequence
+// behind 4000 keys, 8 / 4 heads x 256 f32: 30 us by k_seq_rows, 46 by tiles; 512 behind 1500: 133 and 81).
+// f32 prompts are k_seq_rows's until their tiles fill the chip twice, or once where a window makes them alike:
+// its workgroups are an eighth of the work and even out (8 / 4 heads x 256, 1024 tokens 107 us / 203 by tiles, 4096
+// 731 / 768, but with a window of 512 220 / 146; 32 / 16 heads x 128, 512 tokens 42 / 55, 2048 349 / 214).
 static void choose(SeqArgs& a, int dtype) {
     const bool f32 = dtype == HIP_BRIDGE_F32;
     a.gq = a.nh / a.nkv;
+    const int64_t rows = (int64_t)a.n_tokens * a.gq;
+    auto tiles_of = [&](bool small) { return cdiv(rows, tile_rows_of(dtype, a.D, small)) * a.nkv; };  // if the sequences are even
     // Prompts that leave CUs idle take smaller tiles (64 tokens, 8 / 4 heads x 256 bf16 13.4 -> 10.6 us, 512 of 32
     // / 16 x 128 26 -> 23.5; over the largest, 8192, the larger ones are ahead by 8%).
-    a.tile_rows = tile_rows_of(dtype, a.D, false);
-    if (!a.table && cdiv((int64_t)a.n_tokens * a.gq, a.tile_rows) * a.nkv < 256) a.tile_rows = tile_rows_of(dtype, a.D, true);
+    a.tile_rows = tile_rows_of(dtype, a.D, !a.table && tiles_of(false) < 256);
     const bool single = a.table && !a.cu;  // a token each
     const int few = f32 ? 64 : 16;
-    const int64_t rows = (int64_t)a.n_tokens * a.gq;
-    if ((f32 && !a.table) || rows <= std::max<int64_t>(few, (int64_t)a.n_seqs * few / 2) || (single && a.gq <= few)) a.few_rows = INT32_MAX;
+    const bool short32 = f32 && !a.table && (a.D == 512 || tiles_of(false) < (a.window > 0 ? 256 : 512));
+    if (short32 || rows <= std::max<int64_t>(few, (int64_t)a.n_seqs * few / 2) || (single && a.gq <= few)) a.few_rows = INT32_MAX;
     else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : few;
 
     // A call's splits have one size, whatever the sequences' lengths, which evens out the workgroups of a ragged
@@ -505,15 +507,15 @@ static void choose(SeqArgs& a, int dtype) {
         if (a.n_tokens <= a.n_seqs) a.nsplit = split(16, std::max(least, std::min<int64_t>((1 << 18) / (a.D * (f32 ? 4 : 2)), fill)), a.chunk);
         else if (groups < 1024) a.nsplit = split(16, std::max<int64_t>(fill, 128), a.chunk);
     }
-    if (a.few_rows < INT32_MAX && a.table) {
-        // Chunks whose tiles (if the sequences are even) leave CUs idle: a workgroup to a CU, or a few where
-        // sequences differ. More splits cost more in partial sums than they even out (bf16, 256 tokens behind 8000,
-        // 32 / 16 heads x 128: 63 us at 256 workgroups, 82 at 512, 116 at 1024), but f32 products last longer
-        // (469, 362, 386 us; 15 chunks of up to 162 tokens behind up to 8400: 1550 at 512, 1277 at 2048).
-        const int64_t tiles = cdiv(rows, a.tile_rows) * a.nkv;
-        const int64_t wgs = f32 ? (a.n_seqs > 1 ? 2048 : 512) : (a.n_seqs > 1 ? 512 : 256);
-        const int64_t least = !f32 && a.n_seqs > 1 ? 256 : 128;
-        if (tiles < 256) a.tile_split = split(a.tile_rows, std::max(least, cdiv(tiles * most_keys(a, a.tile_rows), wgs)), a.tile_chunk);
+    if (a.few_rows < INT32_MAX && a.table && tiles_of(false) < 256) {
+        // Chunks whose tiles leave CUs idle: for one sequence as many splits as its tiles have room for at a
+        // workgroup to a CU (256 tokens behind 8000, 32 / 16 heads x 128 bf16: 63 us at 256 workgroups, 82 at
+        // 512, 116 at 1024: partial sums cost more than they even out; f32 213, 362 before it was 256 at the most),
+        // for several, whose lengths differ, two or three to a CU.
+        const int64_t tiles = tiles_of(false), len = most_keys(a, a.tile_rows);
+        const int64_t keys = a.n_seqs == 1 ? std::max<int64_t>(128, cdiv(len, 256 / tiles))
+                                           : std::max<int64_t>(256, cdiv(tiles * len, f32 ? 768 : 512));
+        a.tile_split = split(a.tile_rows, keys, a.tile_chunk);
     }
     a.nparts = std::max(a.nsplit, a.tile_split);
 }

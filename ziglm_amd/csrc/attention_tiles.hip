@@ -477,16 +477,15 @@ static void launch(const SeqArgs& a, hipStream_t s) {
 }
 
 int tile_rows_of(int dtype, int D, bool small) {
-    if (dtype == HIP_BRIDGE_F32 || D == 512) return 64;
+    if (dtype == HIP_BRIDGE_F32 && D < 512) return 128;
+    if (D == 512) return 64;
     return D <= 128 ? (small ? 128 : 256) : small ? 64 : 128;
 }
 
 void launch_tiles(int dtype, const SeqArgs& a, hipStream_t s) {
     const bool small = a.tile_rows < tile_rows_of(dtype, a.D, false);
     if (dtype == HIP_BRIDGE_F32) {
-        if (a.D == 64) launch<float, 64, 16, 4, 32>(a, s);
-        else if (a.D == 128) launch<float, 128, 16, 4, 32>(a, s);
-        else if (a.D == 256) launch<float, 256, 16, 4, 16>(a, s);
+        if (a.D < 512) launch_terms(a, s);
         else launch<float, 512, 16, 8, 16, 2>(a, s);
     } else if (a.D == 512) {
         launch<uint16_t, 512, 16, 8, 32, 2>(a, s);
