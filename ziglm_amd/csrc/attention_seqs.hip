@@ -370,7 +370,7 @@ __global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_
 // they are dropped, not weighted by 0), which leaves one round trip to memory behind the sequence's own.
 constexpr int kMaxSplits = 256;
 constexpr int kJoinWaves = 4;
-constexpr int kJoinFew = 16;
+constexpr int kJoinFew = 16;  // (many heads: up to a wave's 64)
 template <typename T, int D, int W>
 __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
     constexpr int E = D / 64;  // columns of a lane
@@ -465,6 +465,11 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_seq_join(SeqArgs a) {
 
 // ---- host --------------------------------------------------------------------------------------
 
+// Tiles of k_seq_rows, at most: of all sequences, or of those of few rows.
+static int64_t most_few(const SeqArgs& a) {
+    const int64_t all = most_tiles(a, 16);
+    return a.few_rows == INT32_MAX ? all : std::min<int64_t>(all, (int64_t)a.n_seqs * cdiv(a.few_rows, 16));
+}
 // Which kernels a call takes, and the splits of each one's ranges.
 // k_seq_rows reads K and V for 16 query rows; the tile kernels (k_seq_tile; f32 heads up to 256 k_seq_terms)
 // for 64 to 256 that share them. Sequences of few rows (bf16 16, f32 64) are k_seq_rows's, the others the
@@ -501,10 +506,13 @@ static void choose(SeqArgs& a, int dtype) {
         // Decode: half a megabyte of K and V, less where that leaves under 1024 workgroups (16 requests of up to
         // 8192 positions in 8 equal splits each 188 us, in splits of 256 keys 122), down to a block for each wave (one
         // token at 1250, f32: 14.6 us in splits of 64 keys, 19.4 of 128), and no more than 16384 workgroups (whose
-        // partial sums take 17 MB at two heads of 128 to a kv head). Chunks: 1024 workgroups.
-        const int64_t groups = most_tiles(a, 16) * a.nkv, all = most_keys(a, 16) * groups, fill = cdiv(all, 1024);
-        const int64_t least = std::max<int64_t>(f32 ? 64 : 128, cdiv(all, 16384));
-        if (a.n_tokens <= a.n_seqs) a.nsplit = split(16, std::max(least, std::min<int64_t>((1 << 18) / (a.D * (f32 ? 4 : 2)), fill)), a.chunk);
+        // partial sums take 17 MB at two heads of 128 to a kv head). Chunks: 1024 workgroups. Beside tiles: as
+        // decode (a token of a sequence each, mostly), in at most 32 splits, as the tiles' rows pass the join too.
+        const bool decode = a.n_tokens <= a.n_seqs || a.few_rows < INT32_MAX;
+        const int64_t groups = (a.few_rows < INT32_MAX ? (int64_t)a.n_seqs * cdiv(a.gq, 16) : most_tiles(a, 16)) * a.nkv;
+        const int64_t all = most_keys(a, 16) * groups, fill = cdiv(all, 1024);
+        const int64_t least = std::max<int64_t>({f32 ? 64 : 128, cdiv(all, 16384), a.few_rows < INT32_MAX ? cdiv(most_keys(a, 16), 32) : 0});
+        if (decode) a.nsplit = split(16, std::max(least, std::min<int64_t>((1 << 18) / (a.D * (f32 ? 4 : 2)), fill)), a.chunk);
         else if (groups < 1024) a.nsplit = split(16, std::max<int64_t>(fill, 128), a.chunk);
     }
     if (a.few_rows < INT32_MAX && a.table && tiles_of(false) < 256) {
@@ -540,13 +548,13 @@ static size_t workspace_bytes_of(SeqArgs& a, int dtype, bool paged) {
 template <typename T, int D>
 static void launch_rows(const SeqArgs& a, hipStream_t s) {
     if (a.few_rows > 0) {
-        const int64_t grid = most_tiles(a, 16) * a.nkv * a.nsplit;
+        const int64_t grid = most_few(a) * a.nkv * a.nsplit;
         k_seq_rows<T, D><<<(unsigned)grid, row_halves<D>() * kRowWaves * kWave, 0, s>>>(a);
     }
     if (a.few_rows < INT32_MAX) launch_tiles(sizeof(T) == 4 ? HIP_BRIDGE_F32 : HIP_BRIDGE_BF16, a, s);
     if (a.nparts > 1) {
         const int64_t th = (int64_t)a.n_tokens * a.nh;
-        if (a.nparts <= kJoinFew) k_seq_join<T, D, 1><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
+        if (a.nparts <= (th > 2048 ? kWave : kJoinFew)) k_seq_join<T, D, 1><<<(unsigned)cdiv(th, kJoinWaves), kJoinWaves * kWave, 0, s>>>(a);
         else k_seq_join<T, D, kJoinWaves><<<(unsigned)th, kJoinWaves * kWave, 0, s>>>(a);
     }
     check_launch();
