@@ -25,7 +25,9 @@ struct SeqArgs {
     int64_t q_stride, kv_stride;
     int64_t cache_pages;
     int page, page_shift;  // page_shift: log2(page) or -1
-    int max_pages, max_len;
+    int max_pages;
+    int max_len;           // of a sequence, as the caller says: the host's rules go by it
+    int lim;               // positions that there can be: of max_len and of the table's width the smaller
     int n_seqs, n_tokens, nh, nkv, gq, D, window;
     int few_rows;          // sequences of at most this many query rows a kv head are k_seq_rows's, the others k_seq_tile's
     int nsplit, tile_split, nparts;  // splits of k_seq_rows's and k_seq_tile's ranges, the larger of them
@@ -57,7 +59,7 @@ __device__ __forceinline__ Seq seq_of(const SeqArgs& a, int s) {
     q.nq = seq_tokens(a, s, q.tok0);
     if (a.table) {
         q.pos0 = max(a.len[s], 0) - q.nq;
-        q.lim = a.max_len;
+        q.lim = a.lim;
         q.row0 = 0;
         q.pages = a.table + (int64_t)s * a.max_pages;
     } else {

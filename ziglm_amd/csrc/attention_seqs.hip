@@ -647,7 +647,8 @@ void hip_attention_paged(int dtype, const void* q, const void* k_cache, const vo
     a.page = page_size;
     a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
     a.max_pages = max_pages;
-    a.max_len = (int)std::min<int64_t>(max_len, (int64_t)max_pages * page_size);
+    a.max_len = max_len;
+    a.lim = (int)std::min<int64_t>(max_len, (int64_t)max_pages * page_size);
     a.n_seqs = n_seqs;
     a.n_tokens = n_tokens;
     a.nh = n_heads;
