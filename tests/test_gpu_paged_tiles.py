@@ -51,6 +51,14 @@ def test_bf16_prompts(dev, nh, nkv, d, lens, cap, window):
     check_prompts(dev, "bf16", nh, nkv, d, lens, cap, window)
 
 
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (4, 2, 256), (2, 1, 512)])
+@pytest.mark.parametrize("scale,cap", [(1.0, 5.0), (-0.3, 30.0), (1e-6, 1e-3), (1e12, 40.0), (0.05, 1e20)])
+def test_capped_scores(dev, act, nh, nkv, d, scale, cap):
+    """Small scores, scores at the cap, and some of both in one call: a few of a tile's rows are far larger."""
+    check_prompts(dev, act, nh, nkv, d, [200, 70], cap, 0, scale)
+
+
 @pytest.mark.parametrize("nh,nkv,d,lens,cap,window", [
     (16, 16, 64, [3500, 700], 0.0, 0),
     (32, 16, 128, [1500, 2, 600], 0.0, 0),

@@ -32,9 +32,11 @@ struct SeqArgs {
     int few_rows;          // sequences of at most this many query rows a kv head are k_seq_rows's, the others k_seq_tile's
     int nsplit, tile_split, nparts;  // splits of k_seq_rows's and k_seq_tile's ranges, the larger of them
     int chunk, tile_chunk;           // keys of a split
+    int rows_grid, tile_grid;        // workgroups of each
     int tile_rows;         // query rows of a workgroup of k_seq_tile
     float scale, softcap, inv_cap;
     float cap_in;          // 2 log2(e) scale / softcap
+    float cap_small, cap_c[4];  // scores up to this take the series, its coefficients
     float unit;            // of running maxima: log2(e); bf16: log2(e) * |scale|, or log2(e) where soft-capped
 };
 
@@ -135,6 +137,11 @@ inline int64_t most_keys(const SeqArgs& a, int R) {
 // (2^-8); f32 calls take the form that is exact to the last places there too.
 __device__ __forceinline__ float cap_bf16(const SeqArgs& a, float x) {
     return fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.cap_in) + 1.0f), -2.0f * a.softcap, a.softcap);
+}
+// The same where |z| <= 0.35, by tanh's series up to z^7 (off by 62 / 2835 z^9 cap, 2^-19 cap at the most).
+__device__ __forceinline__ float cap_series(const SeqArgs& a, float x) {
+    const float y = x * x;
+    return x * fmaf(y, fmaf(y, fmaf(y, a.cap_c[3], a.cap_c[2]), a.cap_c[1]), a.cap_c[0]);
 }
 
 // 4 consecutive elements as f32

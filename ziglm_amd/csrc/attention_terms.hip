@@ -11,7 +11,7 @@
 // between two barriers.
 // Infinities have no terms. Values of V that are infinite or NaN stay out and go to the rows that see them
 // at the end; keys of K with such values get their scores by a plain dot product.
-#include "attention_seqs.h"
+#include "attention_rows.h"
 
 namespace zl {
 
@@ -52,8 +52,16 @@ __device__ __forceinline__ float over_row4(float v, F f) {
 }
 
 constexpr int kTermWaves = 8, kTermRows = 16 * kTermWaves, kTermKeys = 32;
+// LDS as in k_seq_tile: K's chunks in four planes by their index mod 4, V's rows padded by 32 bytes
+template <int D> struct TermsLds {
+    static constexpr int KS = D / 2 + 16, KP = kTermKeys * KS, VS = 2 * D + 32;
+    static_assert(KP % 256 == 0 && KS / 16 % 2 == 1, "planes");
+    uint8_t k[3][4 * KP], v[3][kTermKeys * VS];
+    uint32_t gap[2], bad[2];  // keys without a row; with infinite or NaN values in K
+    int wild;                 // infinite or NaN values of V were kept out of LDS
+};
 template <int D, bool CAP>
-__global__ __launch_bounds__(kTermWaves * kWave, 2) void k_seq_terms(SeqArgs a) {
+__device__ __forceinline__ void seq_terms(const SeqArgs& a, int id, TermsLds<D>& lds) {
     constexpr int KB = kTermKeys, TH = kTermWaves * kWave;
     constexpr int NQ = D / 32;       // chunks (8 values) of a query row to a lane
     constexpr int NB = D / 16;       // accumulators of the output
@@ -61,15 +69,14 @@ __global__ __launch_bounds__(kTermWaves * kWave, 2) void k_seq_terms(SeqArgs a) 
     constexpr int NC = KB * CR / TH > 0 ? KB * CR / TH : 1;  // of a tile, to a thread
     constexpr int RS = TH / CR;      // rows between a thread's chunks
     constexpr float kSlack = 8.0f;   // log2
-    // LDS as in k_seq_tile: K's chunks in four planes by their index mod 4, V's rows padded by 32 bytes
-    constexpr int KS = D / 2 + 16, KP = KB * KS, VS = 2 * D + 32;
-    static_assert(KP % 256 == 0 && KS / 16 % 2 == 1, "planes");
-    __shared__ __align__(16) uint8_t s_k[3][4 * KP], s_v[3][KB * VS];
-    __shared__ uint32_t s_gap[2], s_bad[2];  // keys without a row; with infinite or NaN values in K
-    __shared__ int s_wild;                   // infinite or NaN values of V were kept out of LDS
+    constexpr int KS = TermsLds<D>::KS, KP = TermsLds<D>::KP, VS = TermsLds<D>::VS;
+    auto& s_k = lds.k;
+    auto& s_v = lds.v;
+    auto& s_gap = lds.gap;
+    auto& s_bad = lds.bad;
+    int& s_wild = lds.wild;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = (int)blockIdx.x;
     const int kvh = id % a.nkv;
     id /= a.nkv;
     const int split = id % a.tile_split;
@@ -379,11 +386,33 @@ __global__ __launch_bounds__(kTermWaves * kWave, 2) void k_seq_terms(SeqArgs a) 
     }
 }
 
+template <int D, bool CAP>
+__global__ __launch_bounds__(kTermWaves * kWave, 2) void k_seq_terms(SeqArgs a) {
+    __shared__ __align__(16) TermsLds<D> lds;
+    seq_terms<D, CAP>(a, (int)blockIdx.x, lds);
+}
+// (as k_seq_both of the bf16 tiles)
+template <int D, bool CAP>
+__global__ __launch_bounds__(kTermWaves * kWave, 2) void k_seq_terms_both(SeqArgs a) {
+    __shared__ __align__(16) union Lds {
+        TermsLds<D> tile;
+        RowsLds<D, kTermWaves> rows;
+    } lds;
+    const int id = (int)blockIdx.x;
+    if (id < a.tile_grid) seq_terms<D, CAP>(a, id, lds.tile);
+    else seq_rows<float, D, kTermWaves>(a, id - a.tile_grid, lds.rows);
+}
+
 template <int D>
 static void launch(const SeqArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)(most_tiles(a, kTermRows) * a.nkv * a.tile_split);
-    if (a.softcap > 0.0f) k_seq_terms<D, true><<<grid, kTermWaves * kWave, 0, s>>>(a);
-    else k_seq_terms<D, false><<<grid, kTermWaves * kWave, 0, s>>>(a);
+    const unsigned grid = (unsigned)(a.tile_grid + a.rows_grid);
+    auto run = [&](auto cap) {
+        constexpr bool CAP = decltype(cap)::value;
+        if (a.rows_grid > 0) k_seq_terms_both<D, CAP><<<grid, kTermWaves * kWave, 0, s>>>(a);
+        else k_seq_terms<D, CAP><<<grid, kTermWaves * kWave, 0, s>>>(a);
+    };
+    if (a.softcap > 0.0f) run(std::true_type{});
+    else run(std::false_type{});
 }
 
 void launch_terms(const SeqArgs& a, hipStream_t s) {

@@ -15,7 +15,7 @@
 // The weights round to bf16 for the second product (half a step, 2^-8 relative, as the output does); their
 // sum takes them unrounded. The running maximum moves only when a row exceeds it by 8 in the exponent
 // (weights up to 2^8 before the final quotient), so that tiles seldom rescale the output.
-#include "attention_seqs.h"
+#include "attention_rows.h"
 
 namespace zl {
 
@@ -50,13 +50,31 @@ __device__ __forceinline__ float over_row(float v, F f) {
     return f(__builtin_bit_cast(float, (unsigned)p[0]), __builtin_bit_cast(float, (unsigned)p[1]));
 }
 
+// LDS is laid out so that no two lanes of a phase meet in a bank (a phase of a 16-byte read has 16 lanes: 0-3,
+// 12-15, 20-27 or 4-11, 16-19, 28-31 of a half wave; of an 8-byte read 32). K: M 32 reads 16 rows at one
+// column in a phase, rows are padded by 16 bytes; M 16 reads 8 rows at one chunk and the others at the
+// next, so the chunks stand in four planes by their index mod 4, rows padded to an odd number of chunks.
+// V: a transposing read has 4 rows and 32 bytes a group of 16 lanes, and in the other group the next 32
+// bytes (M 32: rows padded by 64 bytes) or the next rows (M 16: by 32).
+template <typename T, int D, int M, int NW, int KB, int HV>
+struct TileLds {
+    static constexpr bool BF = sizeof(T) == 2;
+    static constexpr int RB = D * sizeof(T);  // bytes of a row
+    static constexpr int PLANES = M == 32 ? 1 : 4;
+    static constexpr int KS = RB / PLANES + 16, KP = KB * KS, VS = RB + (!BF ? 0 : M == 32 ? 64 : 32);
+    static_assert(M == 32 || (KP % 256 == 0 && KS / 16 % 2 == 1), "planes");
+    static constexpr int GW = (KB + 31) / 32, NU = KB / M * (M * M / 64) / 4;
+    uint8_t k[2][PLANES * KP], v[2][KB * VS];
+    f32x4 x[HV > 1 ? NW : 1][HV > 1 ? NU : 1][HV > 1 ? kWave : 1];  // the halves' sums of the scores
+    uint32_t gap[3][GW];                  // keys without a row
+    int wild;                             // infinite or NaN values were kept out of LDS
+};
 template <typename T, int D, int M, int NW, int KB, int HV, bool CAP>
-__global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
+__device__ __forceinline__ void seq_tile(const SeqArgs& a, int id, TileLds<T, D, M, NW, KB, HV>& lds) {
     typedef typename Mfma<M>::Acc Acc;
     constexpr bool BF = sizeof(T) == 2;
     static_assert(BF || M == 16, "f32 tiles have 16 rows a wave");
     constexpr int EL = 16 / sizeof(T);   // elements of a 16-byte chunk
-    constexpr int RB = D * sizeof(T);    // bytes of a row
     constexpr int G = 64 / M;            // lanes of a query row
     constexpr int DW = D / HV;           // of the head size, a wave's part
     constexpr int RG = NW / HV;          // groups of M query rows
@@ -72,23 +90,15 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     constexpr int RS = TH / CR;          // rows between a thread's chunks
     constexpr float kSlack = 8.0f;       // log2
     static_assert(KB * CR % TH == 0 && TH % CR == 0, "chunks of a tile");
-    // LDS is laid out so that no two lanes of a phase meet in a bank (a phase of a 16-byte read has 16 lanes: 0-3,
-    // 12-15, 20-27 or 4-11, 16-19, 28-31 of a half wave; of an 8-byte read 32). K: M 32 reads 16 rows at one
-    // column in a phase, rows are padded by 16 bytes; M 16 reads 8 rows at one chunk and the others at the
-    // next, so the chunks stand in four planes by their index mod 4, rows padded to an odd number of chunks.
-    // V: a transposing read has 4 rows and 32 bytes a group of 16 lanes, and in the other group the next 32
-    // bytes (M 32: rows padded by 64 bytes) or the next rows (M 16: by 32).
-    constexpr int PLANES = M == 32 ? 1 : 4;
-    constexpr int KS = RB / PLANES + 16, KP = KB * KS, VS = RB + (!BF ? 0 : M == 32 ? 64 : 32);
-    static_assert(M == 32 || (KP % 256 == 0 && KS / 16 % 2 == 1), "planes");
-    __shared__ __align__(16) uint8_t s_k[2][PLANES * KP], s_v[2][KB * VS];
-    constexpr int GW = (KB + 31) / 32;
-    __shared__ uint32_t s_gap[3][GW];       // keys without a row
-    __shared__ f32x4 s_x[HV > 1 ? NW : 1][NU][kWave];  // the halves' sums of the scores
-    __shared__ int s_wild;                  // infinite or NaN values were kept out of LDS
+    typedef TileLds<T, D, M, NW, KB, HV> Lds;
+    constexpr int PLANES = Lds::PLANES, KS = Lds::KS, KP = Lds::KP, VS = Lds::VS, GW = Lds::GW;
+    auto& s_k = lds.k;
+    auto& s_v = lds.v;
+    auto& s_gap = lds.gap;
+    auto& s_x = lds.x;
+    int& s_wild = lds.wild;
     const int tid = threadIdx.x, lane = tid & 63, n = lane % M, h = lane / M;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave / RG;
-    int id = (int)blockIdx.x;
     const int kvh = id % a.nkv;
     id /= a.nkv;
     const int split = id % a.tile_split;
@@ -285,7 +295,19 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
 #pragma unroll
         for (int e = 0; e < NT * SR; ++e) {
             if constexpr (!BF) x[e] *= a.scale;
-            if constexpr (CAP) x[e] = BF ? cap_bf16(a, x[e]) : a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+            if constexpr (CAP && !BF) x[e] = a.softcap * tanh_fast(div_by_uniform(x[e], a.softcap, a.inv_cap));
+        }
+        if constexpr (CAP && BF) {
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < NT * SR; ++e) top = fmaxf(top, fabsf(x[e]));
+            if (__any(!(top <= a.cap_small))) {
+#pragma unroll
+                for (int e = 0; e < NT * SR; ++e) x[e] = cap_bf16(a, x[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < NT * SR; ++e) x[e] = cap_series(a, x[e]);
+            }
         }
         uint32_t gap[GW], some = 0;
 #pragma unroll
@@ -469,11 +491,39 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
     }
 }
 
+template <typename T, int D, int M, int NW, int KB, int HV, bool CAP>
+__global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
+    __shared__ __align__(16) TileLds<T, D, M, NW, KB, HV> lds;
+    seq_tile<T, D, M, NW, KB, HV, CAP>(a, (int)blockIdx.x, lds);
+}
+// Tiles, and behind them 16 rows by as many waves: chunks beside sequences of a token. The rows, which wait for
+// memory, take the CUs that the last tiles leave (24 sequences, three of them chunks of 288 to 492 tokens behind
+// up to 3600, 32 / 16 heads x 128: 187 us in two launches one behind the other, 146 to 174 in one).
+template <typename T, int D, int M, int NW, int KB, int HV, bool CAP>
+__global__ __launch_bounds__(NW * kWave, 2) void k_seq_both(SeqArgs a) {
+    constexpr int W = NW / row_halves<D>();
+    __shared__ __align__(16) union Lds {
+        TileLds<T, D, M, NW, KB, HV> tile;
+        RowsLds<D, W> rows;
+    } lds;
+    const int id = (int)blockIdx.x;
+    if (id < a.tile_grid) seq_tile<T, D, M, NW, KB, HV, CAP>(a, id, lds.tile);
+    else seq_rows<T, D, W>(a, id - a.tile_grid, lds.rows);
+}
+
 template <typename T, int D, int M, int NW, int KB, int HV = 1>
 static void launch(const SeqArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)(most_tiles(a, NW / HV * M) * a.nkv * a.tile_split);
-    if (a.softcap > 0.0f) k_seq_tile<T, D, M, NW, KB, HV, true><<<grid, NW * kWave, 0, s>>>(a);
-    else k_seq_tile<T, D, M, NW, KB, HV, false><<<grid, NW * kWave, 0, s>>>(a);
+    const unsigned grid = (unsigned)(a.tile_grid + a.rows_grid);
+    auto run = [&](auto cap) {
+        constexpr bool CAP = decltype(cap)::value;
+        // (rows stand beside the smaller tiles, where there are two sizes)
+        if constexpr (NW == 4 || HV > 1) {
+            if (a.rows_grid > 0) return k_seq_both<T, D, M, NW, KB, HV, CAP><<<grid, NW * kWave, 0, s>>>(a);
+        }
+        k_seq_tile<T, D, M, NW, KB, HV, CAP><<<grid, NW * kWave, 0, s>>>(a);
+    };
+    if (a.softcap > 0.0f) run(std::true_type{});
+    else run(std::false_type{});
 }
 
 int tile_rows_of(int dtype, int D, bool small) {
