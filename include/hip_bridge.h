@@ -419,8 +419,10 @@ void hip_paged_plan(const int32_t* d_ctx_len /*NULL*/, const int32_t* d_new_len,
  * d_seq_len[s] positions, those of the new tokens included, are in the cache: a token at
  * position p attends to [max(0, p + 1 - window), p] as in hip_attention_decode. q and out
  * [n_tokens][n_heads][head_dim] and the caches are of type dtype (F32 or BF16); sums, softmax
- * and its state are f32; in bf16 the weights round to bf16 for their product with V in calls of
- * many rows. Any n_heads / n_kv_heads, head_dim 64, 128, 256 or 512, any page_size.
+ * and its state are f32. Where a kv head has many query rows, bf16 calls round the weights to bf16
+ * for their product with V, and f32 calls up to head_dim 256 form each product from three bf16 terms
+ * of either factor (exact to 2^-23; factors under 2^-110 lose places). Any n_heads / n_kv_heads,
+ * head_dim 64, 128, 256 or 512, any page_size; at most 2^30 positions.
  * Pages outside [0, cache_pages) hold no keys; a token with no key, at a negative position or
  * at one from min(max_len, max_pages * page_size) on gives zeros; rows of out outside
  * [d_cu[0], d_cu[n_seqs]) stay as they are. d_cu must not fall. Keys that a token does not see

@@ -254,6 +254,32 @@ public:
                             (int)n_tokens, (int)num_heads, (int)num_kv_heads, (int)head_dim, (int)rotary_dim,
                             freq_base, freq_scale, eps, use_unit_offset ? 1 : 0, stream);
     }
+    void pagedPlan(const int32_t* d_ctx_len, const int32_t* d_new_len, size_t n_seqs, size_t page_size,
+                   size_t max_pages, const int32_t* d_free_pages, size_t n_free, const int32_t* d_cursor,
+                   int32_t* d_block_table, size_t n_tokens, int32_t* d_cu, int32_t* d_seq_len, int32_t* d_pos,
+                   int64_t* d_slot, int32_t* d_state) const {
+        hip_paged_plan(d_ctx_len, d_new_len, (int)n_seqs, (int)page_size, (int)max_pages, d_free_pages, (int)n_free,
+                       d_cursor, d_block_table, (int)n_tokens, d_cu, d_seq_len, d_pos, d_slot, d_state, stream);
+    }
+    void attentionPaged(int dtype, const void* d_q, const void* d_k_cache, const void* d_v_cache, void* d_out,
+                        int64_t cache_pages, size_t page_size, int64_t row_stride, const int32_t* d_block_table,
+                        size_t max_pages, const int32_t* d_cu, const int32_t* d_seq_len, size_t n_seqs,
+                        size_t n_tokens, size_t max_len, size_t num_heads, size_t num_kv_heads, size_t head_dim,
+                        float attn_scale, float softcap, size_t sliding_window, void* workspace,
+                        size_t workspace_bytes) const {
+        hip_attention_paged(dtype, d_q, d_k_cache, d_v_cache, d_out, cache_pages, (int)page_size, row_stride,
+                            d_block_table, (int)max_pages, d_cu, d_seq_len, (int)n_seqs, (int)n_tokens, (int)max_len,
+                            (int)num_heads, (int)num_kv_heads, (int)head_dim, attn_scale, softcap,
+                            (int)sliding_window, workspace, workspace_bytes, stream);
+    }
+    void attentionPrompt(int dtype, const void* d_q, const void* d_k, const void* d_v, void* d_out, int64_t q_stride,
+                         int64_t kv_stride, const int32_t* d_cu, size_t n_seqs, size_t n_tokens, size_t num_heads,
+                         size_t num_kv_heads, size_t head_dim, float attn_scale, float softcap,
+                         size_t sliding_window, void* workspace, size_t workspace_bytes) const {
+        hip_attention_prompt(dtype, d_q, d_k, d_v, d_out, q_stride, kv_stride, d_cu, (int)n_seqs, (int)n_tokens,
+                             (int)num_heads, (int)num_kv_heads, (int)head_dim, attn_scale, softcap,
+                             (int)sliding_window, workspace, workspace_bytes, stream);
+    }
     void rmsNormAddRmsNorm(int dtype, void* d_x, const void* d_xb, const float* d_w1, const float* d_w2,
                            void* d_out, int64_t rows, size_t n, float eps, bool use_unit_offset) const {
         hip_rmsnorm_add_rmsnorm(dtype, d_x, d_xb, d_w1, d_w2, d_out, rows, (int)n, eps, use_unit_offset ? 1 : 0,

@@ -93,3 +93,16 @@ def test_workspace_sizes(b):
     for bad in ((B.F32, 0, 1, 100, 8, 4, 256, 0), (B.F32, 1, 0, 100, 8, 4, 256, 0), (B.F32, 1, 1, 0, 8, 4, 256, 0), (B.F32, 1, 1, 100, 8, 3, 256, 0),
                 (B.F32, 1, 1, 100, 8, 4, -1, 0)):
         assert paged(*bad) == 0
+
+
+def test_paged_refuses_positions_past_2_30(b):
+    b.hip_attention_paged(*paged_args(pages=1 << 20, page=1 << 10, most=(1 << 20) + 1, max_len=(1 << 30) + 1))
+    assert b.last_error() == B.EUNSUPPORTED
+
+
+def test_grids_past_the_launch_limit_are_refused(b):
+    """A launch holds under 2^32 threads."""
+    b.hip_attention_paged(*paged_args(cu=None, n=1 << 21, tokens=1 << 21, nh=512, nkv=512, d=64, stride=512 * 64))
+    assert b.last_error() == B.EUNSUPPORTED
+    b.hip_attention_prompt(*prompt_args(dtype=B.BF16, cu=None, n=1, tokens=1 << 21, nh=1000, nkv=1000, d=256, q_stride=256000, kv_stride=256000))
+    assert b.last_error() == B.EUNSUPPORTED

@@ -142,7 +142,7 @@ static void choose(SeqArgs& a, int dtype) {
     auto tiles_of = [&](bool small) { return cdiv(rows, tile_rows_of(dtype, a.D, small)) * a.nkv; };  // if the sequences are even
     const bool single = a.table && !a.cu;  // a token each
     const int few = f32 ? 64 : 16;
-    const bool short32 = f32 && !a.table && (a.D == 512 || tiles_of(false) < (a.window > 0 ? 256 : 512));
+    const bool short32 = f32 && !a.table && (a.D == 512 || tiles_of(false) < (a.window > 0 ? 320 : 512));
     if (short32 || rows <= std::max<int64_t>(few, (int64_t)a.n_seqs * few / 2) || (single && a.gq <= few)) a.few_rows = INT32_MAX;
     else a.few_rows = single || !a.table || a.n_seqs == 1 ? 0 : few;
     // Prompts that leave CUs idle take smaller tiles (64 tokens, 8 / 4 heads x 256 bf16 13.4 -> 10.6 us, 512 of 32
@@ -180,10 +180,11 @@ static void choose(SeqArgs& a, int dtype) {
         // workgroup to a CU (256 tokens behind 8000, 32 / 16 heads x 128 bf16: 63 us at 256 workgroups, 82 at
         // 512, 116 at 1024: partial sums cost more than they even out; f32 213, 362 before it was 256 at the most),
         // for several, whose lengths differ, as many as would give two to a CU if all were as long as the longest
-        // (bf16 up to 256: 512 of the small tiles; the calls above in twice as many 85 us, in these 77).
+        // (of small tiles two and a half: the calls above in four to a CU 85 us, in these 79; in two 77, but others,
+        // whose longest tile is then not split, up to twice as long).
         const int64_t tiles = tiles_of(false), len = most_keys(a, a.tile_rows);
         const int64_t keys = a.n_seqs == 1 ? std::max<int64_t>(128, cdiv(len, 256 / tiles))
-                                           : std::max<int64_t>(256, cdiv(tiles * len, a.tile_rows < tile_rows_of(dtype, a.D, false) ? 256 : 512));
+                                           : std::max<int64_t>(256, cdiv(tiles * len, a.tile_rows < tile_rows_of(dtype, a.D, false) ? 320 : 512));
         a.tile_split = split(a.tile_rows, keys, a.tile_chunk);
     }
     a.nparts = std::max(a.nsplit, a.tile_split);
@@ -295,7 +296,8 @@ void hip_attention_paged(int dtype, const void* q, const void* k_cache, const vo
         set_error(HIP_BRIDGE_EINVAL);
         return;
     }
-    if (cache_pages > INT32_MAX / page_size) {  // cache rows are 32-bit
+    // cache rows are 32-bit, and so are positions, a tile or two past the last included
+    if (cache_pages > INT32_MAX / page_size || std::min<int64_t>(max_len, (int64_t)max_pages * page_size) > 1 << 30) {
         set_error(HIP_BRIDGE_EUNSUPPORTED);
         return;
     }

@@ -547,6 +547,37 @@ pub const HipDevice = struct {
         hip_attention_decode_qk(kv_dtype, d_q, d_k, d_v, q_norm, k_norm, flag(v_norm), d_k_cache, d_v_cache, d_out, @intCast(cache_rows), @intCast(row_stride), d_row_base, @intCast(row_base), d_pos, int(pos_base), int(max_len), int(batch), int(n_heads), int(n_kv_heads), int(head_dim), int(rotary_dim), theta, freq_scale, eps, flag(unit_offset), attn_scale, softcap, int(sliding_window), ws_ptr, ws_len, self.stream);
     }
 
+    /// One step of many requests over a paged KV cache: their new tokens take pages off the free list
+    /// (d_free_pages from *d_cursor on) into the block tables, and every token gets its position and cache
+    /// row (d_pos, d_slot of qkNormRopeKv). d_state: the cursor behind the pages taken, the tokens left out.
+    pub fn pagedPlan(self: *const HipDevice, d_ctx_len: ?[*]const i32, d_new_len: [*]const i32, n_seqs: usize, page_size: usize, max_pages: usize, d_free_pages: ?[*]const i32, n_free: usize, d_cursor: ?[*]const i32, d_block_table: [*]i32, n_tokens: usize, d_cu: [*]i32, d_seq_len: [*]i32, d_pos: [*]i32, d_slot: [*]i64, d_state: [*]i32) void {
+        hip_paged_plan(d_ctx_len, d_new_len, int(n_seqs), int(page_size), int(max_pages), d_free_pages, int(n_free), d_cursor, d_block_table, int(n_tokens), d_cu, d_seq_len, d_pos, d_slot, d_state, self.stream);
+    }
+
+    pub fn attentionPagedWorkspaceBytes(self: *const HipDevice, dtype: c_int, n_seqs: usize, n_tokens: usize, max_len: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, sliding_window: usize) usize {
+        _ = self;
+        return hip_attention_paged_workspace_bytes(dtype, int(n_seqs), int(n_tokens), int(max_len), int(n_heads), int(n_kv_heads), int(head_dim), int(sliding_window));
+    }
+
+    /// Attention of the new tokens of each sequence (one, or a chunk) over its pages of the cache.
+    pub fn attentionPaged(self: *const HipDevice, dtype: c_int, d_q: ?*const anyopaque, d_k_cache: ?*const anyopaque, d_v_cache: ?*const anyopaque, d_out: ?*anyopaque, cache_pages: usize, page_size: usize, row_stride: usize, d_block_table: [*]const i32, max_pages: usize, d_cu: ?[*]const i32, d_seq_len: [*]const i32, n_seqs: usize, n_tokens: usize, max_len: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, attn_scale: f32, softcap: f32, sliding_window: usize, workspace: ?HipBuffer) void {
+        const ws_ptr: ?*anyopaque = if (workspace) |w| w.ptr else null;
+        const ws_len: usize = if (workspace) |w| w.size_bytes else 0;
+        hip_attention_paged(dtype, d_q, d_k_cache, d_v_cache, d_out, @intCast(cache_pages), int(page_size), @intCast(row_stride), d_block_table, int(max_pages), d_cu, d_seq_len, int(n_seqs), int(n_tokens), int(max_len), int(n_heads), int(n_kv_heads), int(head_dim), attn_scale, softcap, int(sliding_window), ws_ptr, ws_len, self.stream);
+    }
+
+    pub fn attentionPromptWorkspaceBytes(self: *const HipDevice, dtype: c_int, n_seqs: usize, n_tokens: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, sliding_window: usize) usize {
+        _ = self;
+        return hip_attention_prompt_workspace_bytes(dtype, int(n_seqs), int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim), int(sliding_window));
+    }
+
+    /// Causal attention of whole prompts, one behind the other (d_cu: where each begins).
+    pub fn attentionPrompt(self: *const HipDevice, dtype: c_int, d_q: ?*const anyopaque, d_k: ?*const anyopaque, d_v: ?*const anyopaque, d_out: ?*anyopaque, q_stride: usize, kv_stride: usize, d_cu: ?[*]const i32, n_seqs: usize, n_tokens: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, attn_scale: f32, softcap: f32, sliding_window: usize, workspace: ?HipBuffer) void {
+        const ws_ptr: ?*anyopaque = if (workspace) |w| w.ptr else null;
+        const ws_len: usize = if (workspace) |w| w.size_bytes else 0;
+        hip_attention_prompt(dtype, d_q, d_k, d_v, d_out, @intCast(q_stride), @intCast(kv_stride), d_cu, int(n_seqs), int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim), attn_scale, softcap, int(sliding_window), ws_ptr, ws_len, self.stream);
+    }
+
     /// GEMV with an input prologue (norm / residual / gelu(x) * r built in the product's
     /// workgroups); up_weights non-null makes it a gate.up GeGLU product.
     pub fn gemvPro(self: *const HipDevice, qtype: GGMLType, d_weights: ?*const anyopaque, d_up_weights: ?*const anyopaque, d_x: [*]const f32, d_y: [*]f32, rows: usize, cols: usize, pro: ?*const HipGemvPrologue) void {
