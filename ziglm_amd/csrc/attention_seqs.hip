@@ -16,8 +16,11 @@ namespace zl {
 constexpr int kRowWaves = 4;
 template <typename T, int D>
 __global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_rows(SeqArgs a) {
-    __shared__ __align__(16) RowsLds<D, kRowWaves> lds;
-    seq_rows<T, D, kRowWaves>(a, (int)blockIdx.x, lds);
+    constexpr int W = kRowWaves;
+    int id = (int)blockIdx.x;
+    __shared__ __align__(16) float s_o[row_slots(D) * 16 * (D + 4)];
+    __shared__ float s_m[W][16], s_l[W][16];
+#include "attention_rows.inl"
 }
 
 // Joins the splits of a (token, head): out = sum_s exp(m_s - M) o_s / sum_s exp(m_s - M) l_s. W waves take
