@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 import seq_ref
-from test_gpu_paged import Paged, TYPES, check, normals, rng_of, values_of
+from test_gpu_paged import MARK, Paged, TYPES, check, normals, rng_of, values_of
+from ziglm_amd.device import Graph
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +195,67 @@ def test_bound_past_the_table(dev, act, nh, nkv, d, ctx, new):
         ws, need = c.workspace(0, most)
         c.check(c.call(d ** -0.5, 0.0, 0, ws, need, most), d ** -0.5, 0.0, 0)
         c.check(c.call(d ** -0.5, 0.0, 0, ws, max(need - 1, 0), most), d ** -0.5, 0.0, 0)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 4, 256), (32, 16, 128), (8, 1, 512)])
+def test_shared_pages(dev, act, nh, nkv, d):
+    """Sequences that share the pages of a common beginning, and one that has a page twice."""
+    c = Paged(dev, 29, act, nh, nkv, d, 16, [400, 500, 90, 300], [1, 120, 1, 40])
+    c.table[1, :20] = c.table[0, :20]
+    c.table[2, :5] = c.table[0, :5]
+    c.table[3, 7] = c.table[3, 2]
+    c.upload()
+    ws, need = c.workspace(0)
+    c.check(c.call(d ** -0.5, 0.0, 0, ws, need), d ** -0.5, 0.0, 0)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 70, 3], [40, 150, 90]])
+def test_first_rows_of_no_sequence(dev, act, new):
+    """d_cu may begin past row 0: the rows before it stay as they are."""
+    c = Paged(dev, 30, act, 8, 4, 128, 16, [300, 33, 5], new).upload()
+    ws, need = c.workspace(0)
+    c.d_cu = dev.from_numpy((c.cu + 3).astype(np.int32))
+    front = c.q[:3].copy()
+    c.q = np.concatenate([front, c.q])[:len(c.q)]  # the pad's rows move to the front
+    c.q64 = np.concatenate([c.q64[:3], c.q64])[:len(c.q64)]
+    c.d_q = dev.from_numpy(c.q)
+    c.pad, pad = 0, c.pad
+    c.tokens += pad
+    raw = c.call(0.1, 0.0, 0, ws, need)
+    mark = values_of(np.full(1, 0xABABABAB, np.uint32).view(c.q.dtype)[:1], act)[0]
+    assert (raw[:3] == mark).all()
+    c.q64 = c.q64[3:]
+    c.check(raw[3:], 0.1, 0.0, 0)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 4, 256), (32, 16, 128), (8, 1, 512)])
+def test_chunks_beside_decode_in_a_graph(dev, act, nh, nkv, d):
+    """Captured, then replayed for other lengths, positions and values in the same buffers."""
+    c = Paged(dev, 31, act, nh, nkv, d, 16, [700, 40, 300], [1, 90, 1]).upload()
+    ws, need = c.workspace(0, 1024)
+    first = c.call(0.06, 0.0, 0, ws, need, 1024)
+    call = (TYPES[act][0], c.d_q, c.d_k, c.d_v, c.out, c.pages, c.page, nkv * d, c.d_table, c.most, c.d_cu, c.d_len, c.n, c.tokens + c.pad, 1024,
+            nh, nkv, d, 0.06, 0.0, 0, ws, need)
+    dev.sync()
+    graph = Graph(dev, lambda: dev.attentionPaged(*call))
+    for shorter in (0, 25, 0, 39):
+        lens = np.array([x - shorter for x in c.len], np.int32)
+        c.d_len.upload(lens)
+        c.out.fill(MARK)
+        dev.sync()
+        graph.launch()
+        dev.sync()
+        got = values_of(c.out.to_numpy(c.q.shape, c.q.dtype)[:c.tokens], act)
+        if not shorter:
+            assert np.array_equal(got, first)
+            continue
+        for s in range(c.n):
+            rows = c.rows(s)[:lens[s]]
+            K, V = (values_of(x[rows], act).reshape(-1, nkv, d) for x in (c.kc, c.vc))
+            a = c.cu[s]
+            ref, tol = seq_ref.attend_f64(c.q64[a:a + c.new[s]], K, V, c.ctx[s] - shorter, 0.06, bf16=act == "bf16")
+            check(got[a:a + c.new[s]], ref, tol, (shorter, s))
+    graph.destroy()
