@@ -27,7 +27,8 @@ __global__ __launch_bounds__(row_halves<D>() * kRowWaves * kWave, 2) void k_seq_
 // a head, wave w splits w, w + W, ...: four where there can be many splits, one where there are few
 // (and a workgroup four heads). The row's splits are those of the tile that formed them. The maxima
 // and the first sums are requested before their number is known (slots behind it hold anything:
-// they are dropped, not weighted by 0), which leaves one round trip to memory behind the sequence's own.
+// they are dropped, not weighted by 0), which leaves one round trip to memory behind the sequence's own
+// (one token: 3.9 us of its 14.4; 1330 tokens of 32 heads x 128 beside chunks 23 of 245, bound by the sums' bytes).
 constexpr int kMaxSplits = 256;
 constexpr int kJoinWaves = 4;
 constexpr int kJoinFew = 16;  // (many heads: up to a wave's 64)

@@ -15,6 +15,10 @@
 // The weights round to bf16 for the second product (half a step, 2^-8 relative, as the output does); their
 // sum takes them unrounded. The running maximum moves only when a row exceeds it by 8 in the exponent
 // (weights up to 2^8 before the final quotient), so that tiles seldom rescale the output.
+// Heads of 64 and 128 are bound by the softmax's vector instructions beside the MFMAs (a prompt of 8192, 32 / 16
+// heads x 128: 562 us, 978 TFLOP/s, matrix cores 38% and vector units 46% busy; 4096: 154 us), heads of 256
+// and 512 by LDS, whose rows 16-row waves read for half the products (4096, 8 / 4 x 256: 166 us, 414 TFLOP/s; 2048,
+// 8 / 1 x 512: 136 us). 32 rows a wave do not fit at 256 (61 us against 38.7 for 512 tokens behind 1500).
 #include "attention_rows.h"
 
 namespace zl {
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_seq_tile(SeqArgs a) {
 }
 // Tiles, and behind them 16 rows by as many waves: chunks beside sequences of a token. The rows, which wait for
 // memory, take the CUs that the last tiles leave (24 sequences, three of them chunks of 288 to 492 tokens behind
-// up to 3600, 32 / 16 heads x 128: 187 us in two launches one behind the other, 146 to 174 in one).
+// up to 3600, 32 / 16 heads x 128: 187 us in two launches one behind the other, 149 in one).
 template <typename T, int D, int M, int NW, int KB, int HV, bool CAP>
 __global__ __launch_bounds__(NW * kWave, 2) void k_seq_both(SeqArgs a) {
     constexpr int W = NW / row_halves<D>();
