@@ -12,7 +12,7 @@
 // Infinities have no terms. Values of V that are infinite or NaN stay out and go to the rows that see them
 // at the end; keys of K with such values get their scores by a plain dot product.
 // It waits at its two barriers a tile, a workgroup to a CU (512 tokens behind 1501, 8 / 4 heads x 256: 75 us with the
-// join, matrix cores 25% and vector units 29% busy, by the f32 MFMA 146; a prompt of 4096, 32 / 16 x 128: 778 us,
+// join, matrix cores 25% and vector units 29% busy, by the f32 MFMA 109; a prompt of 4096, 32 / 16 x 128: 778 us,
 // 177 TFLOP/s, which is past the 153 that a large f32 matrix product reaches).
 #include "attention_rows.h"
 

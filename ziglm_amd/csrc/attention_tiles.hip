@@ -18,7 +18,7 @@
 // Heads of 64 and 128 are bound by the softmax's vector instructions beside the MFMAs (a prompt of 8192, 32 / 16
 // heads x 128: 562 us, 978 TFLOP/s, matrix cores 38% and vector units 46% busy; 4096: 154 us), heads of 256
 // and 512 by LDS, whose rows 16-row waves read for half the products (4096, 8 / 4 x 256: 166 us, 414 TFLOP/s; 2048,
-// 8 / 1 x 512: 136 us). 32 rows a wave do not fit at 256 (61 us against 38.7 for 512 tokens behind 1500).
+// 8 / 1 x 512: 136 us). 32 rows a wave do not fit at 256 (five prompts, 4099 tokens, window 512: 61 us against 38.7).
 #include "attention_rows.h"
 
 namespace zl {
